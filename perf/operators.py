@@ -259,7 +259,7 @@ def _plan(s):
     held = (past + page - 1) // page
     after = (past + new_rows + page - 1) // page
     sound = (past >= 0) & (held <= width)
-    in_table, in_rows = after <= width, starts[1:] <= rows
+    in_table, in_rows = after <= width, (starts[1:] <= rows) | (new_rows == 0)
     asks = grows & sound & in_table & in_rows
     need = torch.where(asks, after - held, 0)
     upto = need.cumsum(0)
