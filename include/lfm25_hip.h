@@ -555,6 +555,104 @@ int lfm25_batch_decode_hidden(const lfm25_batch* b, const int32_t* tokens_in, co
 int lfm25_batch_linear(const uint16_t* x, const uint16_t* w, uint16_t* y, int32_t rows, int32_t n, int32_t k,
                        lfm25_stream_t stream);
 
+/* ------------------------------------------------------------ paged 8-bit KV cache
+ *
+ * A cache for many requests whose memory goes by what they hold: a pool of
+ * `pages` pages of `page` positions (16, 32, 64, 128 or 256), one byte a
+ * value, with one FP32 scale per page and KV head. No counterpart in the
+ * reference, whose caches are BF16 and contiguous per sequence (its chunked
+ * cache, lfm25_attention_chunked_cache_kernel.py:16-18, is the nearest: 64
+ * positions a block, all of one sequence).
+ *
+ *   key_cache    [pages x kv_heads x page x head_dim]
+ *   value_cache  [pages x kv_heads x head_dim x page]
+ *   key_scales, value_scales  FP32 [pages x kv_heads]
+ *
+ * in int8 (-127 .. 127) or FP8 e4m3 (finite codes), 16-byte aligned; a value
+ * stands for code * scale; scales are not negative. head_dim is 64 or 128. A
+ * block table, int32 [requests x width], gives request b's pages in the order
+ * of its positions; entries past what it holds may be anything. A pass brings
+ * rows, packed request after request: request b's are rows row_starts[b] ..
+ * row_starts[b + 1), at positions past[b], past[b] + 1, ... A page may be in
+ * several tables (a shared beginning), but rows may be appended to it for one
+ * request only. The three calls of a pass, in order on one stream, are
+ * lfm25_kv8_plan, lfm25_kv8_append (for each layer's pool; the page numbers
+ * are the same) and lfm25_kv8_attention; all may be captured into a graph,
+ * whose replays read the lengths of the moment. */
+#define LFM25_KV8_INT8 0
+#define LFM25_KV8_FP8 1
+#define LFM25_KV8_MAX_REQUESTS 4096
+
+/* Why lfm25_kv8_plan refused a request (status[b]; 0: it did not). */
+#define LFM25_KV8_LENGTH 1 /* past[b] is negative, or more than the table's row holds */
+#define LFM25_KV8_TABLE 2  /* the new rows go past the table's row */
+#define LFM25_KV8_POOL 4   /* no free pages for the new rows, or (an ending request) no room in the ring */
+#define LFM25_KV8_ROWS 8   /* the new rows go past `rows` */
+
+/* Pages, row offsets and slots for a pass, from lengths on the device. past,
+ * counts: int32 [requests], positions held and new rows; counts[b] < 0 ends
+ * request b. free_pages: int32 [ring], a ring of free page numbers; cursor:
+ * int64 [2], entries taken from it and given to it so far, so that entries
+ * cursor[0] .. cursor[1] (modulo ring) are free.
+ *
+ * Each request in order takes the pages that its new rows need from the ring
+ * (they go to its block_table row behind those it holds), or, ending, gives
+ * its pages back (behind cursor[1]; they are free from the next call on, and
+ * its table row is left as it is). row_starts: int32 [requests + 1], the sum
+ * of the counts before each request (those of refused ones too: its rows are
+ * in the pass). slots: int32 [rows], page * page size + position within it of
+ * each row; -1 for a refused request's rows and for those behind the last.
+ * A request is served whole or refused with its reason in status (int32
+ * [requests]) and nothing taken; once the pool is short, requests behind that
+ * still find what they need only if they need no page. next_cursor: int64
+ * [2], the cursor after the call; it may be cursor itself. A cursor whose
+ * difference is not in [0, ring] is taken for an empty pool. */
+int lfm25_kv8_plan(const int32_t* past, const int32_t* counts, int32_t requests, int32_t* block_table, int32_t width,
+                   int32_t* free_pages, int32_t ring, const int64_t* cursor, int32_t* row_starts, int32_t* slots,
+                   int32_t rows, int64_t* next_cursor, int32_t* status, int32_t page, lfm25_stream_t stream);
+
+/* New keys and values into the cache: row r ([kv_heads x head_dim] BF16 at
+ * keys + r * key_stride, in elements, a multiple of 8; values alike) goes to
+ * slots[r]; rows whose slot is outside the pool are left out. Rows of one
+ * page follow one another, at consecutive slots (as lfm25_kv8_plan gives
+ * them); one page in two separate runs of a call is an error that is not
+ * found.
+ *
+ * A page's scale for a head becomes the smallest power of two (2^-120 at
+ * least) that brings the largest new magnitude to 127 (int8) or 448 (FP8) or
+ * below, and no smaller than before when the rows do not begin at the page's
+ * first position; then what the page holds is rounded again to the new scale.
+ * Codes are round-to-nearest-even of value / scale; magnitudes past 1.875 *
+ * 2^127 count as that. A value that is not finite makes the scale NaN, until
+ * the page is begun anew. */
+int lfm25_kv8_append(const uint16_t* keys, int64_t key_stride, const uint16_t* values, int64_t value_stride,
+                     const int32_t* slots, int32_t rows, void* key_cache, void* value_cache, float* key_scales,
+                     float* value_scales, int32_t pages, int32_t page, int32_t kv_heads, int32_t head_dim,
+                     int32_t format, lfm25_stream_t stream);
+
+/* Causal attention of the pass's rows over the cache: row i of request b
+ * attends to positions 0 .. past[b] + i (its own included: append first) with
+ * softmax(scale * q . k). query: BF16 rows [heads x head_dim] at query + r *
+ * query_stride (elements, a multiple of 8); output [rows x heads x head_dim]
+ * BF16, contiguous; heads = kv_heads * group, group in [1, 16], query head j
+ * with KV head j / group. FP32 scores, sums and statistics. max_rows: no
+ * request brings more rows. A row that sees no position (past[b] + i < 0) is
+ * zero; rows behind row_starts[requests] are left as they were. status (int32,
+ * may be NULL), set and never cleared here: bit 0, a page number outside the
+ * pool or a position past the table: rows that attend to it are NaN; bit 1,
+ * a request with row offsets outside the rows or out of order, or with more
+ * than max_rows rows: its rows are left as they were. workspace:
+ * lfm25_kv8_attention_workspace_bytes() of the same arguments, 16-byte
+ * aligned, contents ignored (NULL if that is 0); calls sharing one must not
+ * overlap. output must not overlap the inputs. */
+size_t lfm25_kv8_attention_workspace_bytes(int32_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                           int32_t requests, int32_t max_rows, int32_t width, int32_t page);
+int lfm25_kv8_attention(const uint16_t* query, int64_t query_stride, const void* key_cache, const void* value_cache,
+                        const float* key_scales, const float* value_scales, const int32_t* block_table, int32_t width,
+                        const int32_t* past, const int32_t* row_starts, int32_t requests, uint16_t* output, int32_t rows,
+                        int32_t heads, int32_t max_rows, float scale, int32_t pages, int32_t page, int32_t kv_heads,
+                        int32_t head_dim, int32_t format, int32_t* status, void* workspace, lfm25_stream_t stream);
+
 /* ------------------------------------------------------------ Parakeet encoder
  *
  * The FastConformer encoder of the reference's all-NPU Parakeet path

@@ -21,7 +21,7 @@ CSRC = HERE / "csrc"
 INCLUDE = HERE.parent / "include"
 LIBRARY = HERE / "liblfm25_hip.so"
 SOURCES = ("lfm25_ops.hip", "lfm25_compat.hip", "lfm25_layer.hip", "lfm25_decode.hip", "lfm25_batch.hip",
-           "lfm25_prompt.hip", "lfm25_parakeet.hip")
+           "lfm25_prompt.hip", "lfm25_kv8.hip", "lfm25_parakeet.hip")
 ARCH = os.environ.get("LFM25_OFFLOAD_ARCH", "gfx950")
 
 

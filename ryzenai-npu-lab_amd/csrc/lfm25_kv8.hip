@@ -1,0 +1,1252 @@
+// The paged 8-bit KV cache on gfx950: pages and slots for a pass (k_kv8_plan),
+// the quantizing append (k_kv8_append) and causal attention over the pages
+// (k_kv8_attend_narrow, k_kv8_attend_wide, k_kv8_combine).
+//
+// Layout: a pool of pages of `page` positions. Keys [pages][kv][page][dim],
+// values [pages][kv][dim][page] (a value row of one dimension is contiguous
+// along the positions, which is the order the matrix cores read it in), one
+// byte each (int8 or FP8 e4m3), and one FP32 scale per page and KV head for
+// keys and for values. A value stands for code * scale.
+#include <algorithm>
+#include <cmath>
+
+#include "lfm25_host.h"
+#include "lfm25_device.h"
+
+namespace lfm25 {
+namespace {
+
+constexpr int kMaxRequests = LFM25_KV8_MAX_REQUESTS;
+constexpr int kStatusPage = 1;  // attention: a table entry outside the pool, or a position past the table
+constexpr int kStatusRows = 2;  // attention: row offsets outside the rows, or more rows than max_rows
+
+// ------------------------------------------------------------------ plan
+//
+// With P the page size: held = ceil(past / P), after = ceil((past + count) /
+// P), need = after - held; an exclusive sum of the needs indexes the free
+// ring. One block, so that the cursor may be updated in place and every
+// read of the ring comes before the cursor moves; requests four to a thread,
+// rows and pages one to a thread, each finding its request by bisection of
+// the sums in LDS.
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanEach = kMaxRequests / kPlanThreads;
+
+struct Sums {
+  int64_t a, b;
+};
+
+// Exclusive sums over the block's threads; *total = the whole sums.
+__device__ __forceinline__ Sums block_sums(Sums v, Sums* waves, Sums* total) {
+  Sums s = v;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int64_t a = __shfl_up(s.a, d, kWave), b = __shfl_up(s.b, d, kWave);
+    if (lane_id() >= d) s.a += a, s.b += b;
+  }
+  __syncthreads();  // the sums of a call before are read
+  if (lane_id() == kWave - 1) waves[wave_id()] = s;
+  __syncthreads();
+  Sums before{0, 0}, all{0, 0};
+  for (int w = 0; w < kPlanThreads / kWave; ++w) {
+    if (w == wave_id()) before = all;
+    all.a += waves[w].a, all.b += waves[w].b;
+  }
+  *total = all;
+  return Sums{before.a + s.a - v.a, before.b + s.b - v.b};
+}
+
+// The last index i of at[0 .. n] with at[i] <= x (at[0] = 0 <= x).
+__device__ __forceinline__ int last_not_above(const int* at, int n, int x) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (at[mid] <= x) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+struct PlanShared {
+  Sums waves[kPlanThreads / kWave];
+  int starts[kMaxRequests + 1];  // first row of each request
+  int takes[kMaxRequests + 1];   // pages taken before each request
+  int gives[kMaxRequests + 1];   // pages given back before each request
+  uint8_t status[kMaxRequests];
+};
+
+__device__ __forceinline__ int clamp_int(int64_t v) { return v > INT32_MAX ? INT32_MAX : (int)v; }
+
+__global__ void __launch_bounds__(kPlanThreads) k_kv8_plan(const int* __restrict__ past, const int* __restrict__ counts,
+                                                           int n, int* table, int width, int* ring, int ring_n,
+                                                           const int64_t* cursor, int* __restrict__ row_starts,
+                                                           int* __restrict__ slots, int rows, int64_t* next_cursor,
+                                                           int* __restrict__ status, int shift) {
+  __shared__ PlanShared sh;
+  const int t = threadIdx.x, page = 1 << shift;
+  const int64_t taken = cursor[0], given = cursor[1];
+  const int64_t window = given - taken;
+  const bool sound_ring = taken >= 0 && window >= 0 && window <= ring_n;
+  const int64_t free = sound_ring ? window : 0;
+  const int each = (n + kPlanThreads - 1) / kPlanThreads;
+  int p[kPlanEach], c[kPlanEach];
+  Sums v{0, 0}, total;
+  for (int j = 0; j < kPlanEach; ++j) {
+    const int b = t * each + j;
+    p[j] = c[j] = 0;
+    if (j < each && b < n) {
+      p[j] = past[b];
+      c[j] = counts[b];
+      v.a += c[j] > 0 ? c[j] : 0;
+    }
+  }
+  int64_t row = block_sums(v, sh.waves, &total).a;
+  const int64_t all_rows = total.a;
+  // what each request asks for; the row offsets decide which fit the rows
+  int need[kPlanEach], give[kPlanEach], why[kPlanEach];
+  v = Sums{0, 0};
+  for (int j = 0; j < kPlanEach; ++j) {
+    const int b = t * each + j;
+    need[j] = give[j] = why[j] = 0;
+    if (j >= each || b >= n) continue;
+    sh.starts[b] = clamp_int(row);
+    const int64_t held = ((int64_t)p[j] + page - 1) >> shift;
+    row += c[j] > 0 ? c[j] : 0;
+    if (p[j] < 0 || held > width) {
+      why[j] = LFM25_KV8_LENGTH;
+    } else if (c[j] < 0) {
+      give[j] = (int)held;
+    } else {
+      const int64_t after = ((int64_t)p[j] + c[j] + page - 1) >> shift;
+      if (after > width) why[j] = LFM25_KV8_TABLE;
+      else if (c[j] > 0 && row > rows) why[j] = LFM25_KV8_ROWS;
+      else need[j] = (int)(after - held);
+    }
+    v.a += need[j], v.b += give[j];
+  }
+  const Sums before = block_sums(v, sh.waves, &total);
+  int64_t take = before.a, back = before.b;
+  // The sums only grow, so every request after the first that the pool cannot
+  // serve is refused too, if it needs a page: the first `mine` pages go to
+  // the requests served, in order.
+  v = Sums{0, 0};
+  for (int j = 0; j < kPlanEach; ++j) {
+    const int b = t * each + j;
+    if (j >= each || b >= n) continue;
+    sh.takes[b] = clamp_int(take);
+    sh.gives[b] = clamp_int(back);
+    take += need[j], back += give[j];
+    if (need[j] > 0 && take > free) why[j] = LFM25_KV8_POOL;
+    if (give[j] > 0 && (!sound_ring || free + back > ring_n)) why[j] = LFM25_KV8_POOL;
+    if (!why[j]) v.a += need[j], v.b += give[j];
+    sh.status[b] = (uint8_t)why[j];
+    status[b] = why[j];
+    row_starts[b] = sh.starts[b];
+  }
+  if (t == 0) {
+    sh.starts[n] = clamp_int(all_rows);
+    sh.takes[n] = clamp_int(total.a);
+    sh.gives[n] = clamp_int(total.b);
+    row_starts[n] = clamp_int(all_rows);
+  }
+  block_sums(v, sh.waves, &total);  // (its barriers also publish the sums above)
+  const int mine = (int)total.a, returned = (int)total.b;
+  const int head = sound_ring ? (int)(taken % ring_n) : 0, tail = sound_ring ? (int)(given % ring_n) : 0;
+  const auto at = [&](int from, int k) {  // ring entry k past `from`, k <= ring_n
+    const int64_t i = (int64_t)from + k;
+    return (int)(i >= ring_n ? i - ring_n : i);
+  };
+  for (int k = t; k < mine; k += kPlanThreads) {
+    const int b = last_not_above(sh.takes, n, k);
+    const int held = (int)(((int64_t)past[b] + page - 1) >> shift);
+    table[(size_t)b * width + held + (k - sh.takes[b])] = ring[at(head, k)];
+  }
+  for (int k = t; k < returned; k += kPlanThreads) {
+    const int b = last_not_above(sh.gives, n, k);
+    ring[at(tail, k)] = table[(size_t)b * width + (k - sh.gives[b])];
+  }
+  for (int r = t; r < rows; r += kPlanThreads) {
+    int slot = -1;
+    if (r < all_rows) {
+      const int b = last_not_above(sh.starts, n, r);
+      if (b < n && !sh.status[b]) {
+        const int first = past[b], pos = first + (r - sh.starts[b]);
+        const int held = (int)(((int64_t)first + page - 1) >> shift), i = pos >> shift;
+        const int id = i < held ? table[(size_t)b * width + i] : ring[at(head, sh.takes[b] + i - held)];
+        if (id >= 0 && id <= (INT32_MAX >> shift)) slot = id * page + (pos & (page - 1));
+      }
+    }
+    slots[r] = slot;
+  }
+  if (t == 0) {
+    next_cursor[0] = taken + mine;
+    next_cursor[1] = given + returned;
+  }
+}
+
+// ------------------------------------------------------------------ 8-bit codes
+
+template <bool kFp8>
+struct Code;
+
+// int8: -127 .. 127, to the nearest, ties to even.
+template <>
+struct Code<false> {
+  static constexpr float kMost = 127.0f;
+  static constexpr int kMostExponent = 6;     // 127 = 1.984375 * 2^6
+  static constexpr uint32_t kMostMantissa = 0x7eu;  // the BF16 mantissa bits of 1.984375
+  __device__ static __forceinline__ uint32_t one(float v) {
+    return (uint32_t)(int)rintf(fminf(fmaxf(v, -kMost), kMost)) & 0xffu;
+  }
+  __device__ static __forceinline__ uint32_t four(float a, float b, float c, float d) {
+    return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
+  }
+  __device__ static __forceinline__ void values(uint32_t w, float (&f)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = (float)(int8_t)(w >> (8 * i));
+  }
+  // four codes as BF16 pairs; every code is a BF16 number, so the upper half
+  // of its FP32 form is exact
+  __device__ static __forceinline__ void pairs(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    float f[4];
+    values(w, f);
+    lo = __builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), 0x07060302u);
+    hi = __builtin_amdgcn_perm(__float_as_uint(f[3]), __float_as_uint(f[2]), 0x07060302u);
+  }
+};
+
+// FP8 e4m3 (finite values up to 448), to the nearest, ties to even.
+template <>
+struct Code<true> {
+  static constexpr float kMost = 448.0f;
+  static constexpr int kMostExponent = 8;     // 448 = 1.75 * 2^8
+  static constexpr uint32_t kMostMantissa = 0x60u;  // the BF16 mantissa bits of 1.75
+  __device__ static __forceinline__ float in_range(float v) { return fminf(fmaxf(v, -kMost), kMost); }
+  __device__ static __forceinline__ uint32_t one(float v) {
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(in_range(v), 0.0f, 0, false) & 0xffu;
+  }
+  __device__ static __forceinline__ uint32_t four(float a, float b, float c, float d) {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(in_range(a), in_range(b), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(in_range(c), in_range(d), lo, true);
+  }
+  __device__ static __forceinline__ void values(uint32_t w, float (&f)[4]) {
+    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    f[0] = a[0], f[1] = a[1], f[2] = b[0], f[3] = b[1];
+  }
+  __device__ static __forceinline__ void pairs(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, false));
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, true));
+  }
+};
+
+// ------------------------------------------------------------------ append
+
+struct Append {
+  const uint16_t* x[2];  // keys, values: rows of kv * dim BF16 values
+  int64_t stride[2];     // elements between rows
+  uint8_t* cache[2];
+  float* scales[2];
+  const int* slots;
+  int rows, kv, pages, shift, chunk;
+};
+
+constexpr int kAppendThreads = 256;
+constexpr float kLargest = 0x1.ep127f;  // 1.875 * 2^127: its code times its scale is finite in both formats
+constexpr int kSmallestScale = -120;
+
+// The smallest power of two s with largest <= kMost * s, from the largest
+// value's BF16 magnitude bits (its exponent, plus one where its mantissa is
+// past kMost's). An FP8 code keeps its 3 mantissa bits at any such s, and
+// both formats move to a larger s by an exact power of two, so that what is
+// stored does not depend on how rows were divided among calls but for the
+// rounding of what falls off the end (at most one step in all, 1/2 + 1/4 + ..).
+template <bool kFp8>
+__device__ __forceinline__ float scale_for(uint32_t largest) {
+  int e = (int)(largest >> 7) - 127 - Code<kFp8>::kMostExponent + ((largest & 0x7fu) > Code<kFp8>::kMostMantissa ? 1 : 0);
+  if (e < kSmallestScale) e = kSmallestScale;
+  return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
+struct AppendShared {
+  uint32_t largest[kAppendThreads / kWave];
+};
+
+// One run of rows [r0, r0 + len) (positions off .. off + len of one page) of
+// one KV head, keys (which = 0) or values, by `team` waves, this one number
+// `member`. Teams of more than one wave meet at block barriers.
+template <int D, bool kFp8, int kTeam>
+__device__ __forceinline__ void append_run(const Append& a, AppendShared& sh, int which, int member, int h, int id, int off,
+                                           int r0, int len) {
+  const int l = lane_id(), tid = member * kWave + l, threads = kTeam * kWave, page = 1 << a.shift;
+  const size_t region = ((size_t)id * a.kv + h) * (size_t)D << a.shift;
+  uint8_t* const cache = a.cache[which] + region;
+  float* const scale_at = a.scales[which] + (size_t)id * a.kv + h;
+  const uint16_t* const x = a.x[which] + (size_t)r0 * a.stride[which] + (size_t)h * D;
+  const int64_t stride = a.stride[which];
+  const float old = off > 0 ? *scale_at : 0.0f;
+  // the largest magnitude, on the BF16 bits: what is not finite is past 0x7f80
+  constexpr int kPer = D / 8;
+  uint32_t largest = 0;
+  for (int u = tid; u < len * kPer; u += threads) {
+    const Pack8 w = load8(x + (u / kPer) * stride + 8 * (u % kPer));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) largest = max(largest, max(w.w[i] & 0x7fffu, (w.w[i] >> 16) & 0x7fffu));
+  }
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) largest = max(largest, (uint32_t)__shfl_xor((int)largest, d, kWave));
+  if (kTeam > 1) {
+    if (l == 0) sh.largest[which * kTeam + member] = largest;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kTeam; ++i) largest = max(largest, sh.largest[which * kTeam + i]);
+    __syncthreads();  // read before the next run writes
+  }
+  const bool lost = largest >= 0x7f80u || old != old;  // not finite, or the page was lost before
+  const float scale = lost ? __uint_as_float(0x7fc00000u) : fmaxf(old, scale_for<kFp8>(largest));
+  const bool grows = !lost && off > 0 && scale > old;
+  const float ratio = grows ? old / scale : 1.0f;
+  if (tid == 0 && (off == 0 || lost || grows)) *scale_at = scale;
+  const auto code_of = [&](uint32_t bits16) {
+    const float v = fminf(fmaxf(bf16_to_f32(bits16), -kLargest), kLargest);
+    return lost ? 0.0f : v / scale;
+  };
+  const auto moved = [&](uint32_t w) {
+    float f[4];
+    Code<kFp8>::values(w, f);
+    return Code<kFp8>::four(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
+  };
+  if (which == 0) {
+    for (int u = tid; u < len * kPer; u += threads) {
+      const int r = u / kPer, d = 8 * (u % kPer);
+      const Pack8 w = load8(x + r * stride + d);
+      uint2 c;
+      c.x = Code<kFp8>::four(code_of(w.w[0] & 0xffffu), code_of(w.w[0] >> 16), code_of(w.w[1] & 0xffffu), code_of(w.w[1] >> 16));
+      c.y = Code<kFp8>::four(code_of(w.w[2] & 0xffffu), code_of(w.w[2] >> 16), code_of(w.w[3] & 0xffffu), code_of(w.w[3] >> 16));
+      *reinterpret_cast<uint2*>(cache + (size_t)(off + r) * D + d) = c;
+    }
+    if (grows) {
+      for (int u = tid; u < off * (D / 16); u += threads) {
+        uint4 w = *reinterpret_cast<const uint4*>(cache + (size_t)u * 16);
+        w.x = moved(w.x), w.y = moved(w.y), w.z = moved(w.z), w.w = moved(w.w);
+        *reinterpret_cast<uint4*>(cache + (size_t)u * 16) = w;
+      }
+    }
+    return;
+  }
+  // Values: a thread owns two dimensions of 16 positions (32 bytes), so no
+  // byte has two writers: whole new segments and changed old ones as 16-byte
+  // stores, a few new positions as bytes.
+  const int s0 = grows ? 0 : off >> 4, s1 = (off + len + 15) >> 4;
+  for (int u = tid; u < (s1 - s0) * (D / 2); u += threads) {
+    const int seg = s0 + u / (D / 2), d = 2 * (u % (D / 2)), p0 = 16 * seg;
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = p0 + i - off;
+      w[i] = r >= 0 && r < len ? *reinterpret_cast<const uint32_t*>(x + r * stride + d) : 0u;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      uint8_t* const at = cache + (((size_t)(d + k)) << a.shift) + p0;
+      uint32_t c[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = code_of(k ? w[4 * i + j] >> 16 : w[4 * i + j] & 0xffffu);
+        c[i] = Code<kFp8>::four(f[0], f[1], f[2], f[3]);
+      }
+      const bool whole = p0 >= off && p0 + 16 <= off + len;
+      if (!whole && grows && p0 < off) {  // old positions before `off`, perhaps new ones behind them
+        const uint4 o = *reinterpret_cast<const uint4*>(at);
+        const uint32_t was[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t m = moved(was[i]);
+          uint32_t r = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int pos = p0 + 4 * i + j;
+            const uint32_t from = pos < off ? m : pos < off + len ? c[i] : was[i];
+            r |= from & (0xffu << (8 * j));
+          }
+          c[i] = r;
+        }
+      }
+      if (whole || (grows && p0 < off)) {
+        *reinterpret_cast<uint4*>(at) = uint4{c[0], c[1], c[2], c[3]};
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (p0 + i >= off && p0 + i < off + len) at[i] = (uint8_t)(c[i / 4] >> (8 * (i % 4)));
+      }
+    }
+  }
+  (void)page;
+}
+
+// A run is consecutive rows whose slots follow one another within one page;
+// each is handled whole, where it begins, so that its page's scale has one
+// writer. Block (c, h): the runs that begin in rows [chunk c, chunk (c + 1))
+// of KV head h; long runs by the whole block (two waves for the keys, two for
+// the values), short ones by a wave for each of the two.
+template <int D, bool kFp8>
+__global__ void __launch_bounds__(kAppendThreads) k_kv8_append(const Append a) {
+  __shared__ AppendShared sh;
+  const int h = blockIdx.y, w = wave_id(), l = lane_id(), page = 1 << a.shift;
+  const int most = a.pages << a.shift;  // (the host checks that it is an int)
+  const int c0 = blockIdx.x * a.chunk;
+  int turn = 0;
+  for (int r0 = c0; r0 < min(c0 + a.chunk, a.rows); ++r0) {
+    const int slot = a.slots[r0];
+    if (slot < 0 || slot >= most) continue;
+    const int off = slot & (page - 1);
+    if (off != 0 && r0 > 0 && a.slots[r0 - 1] == slot - 1) continue;  // not where its run begins
+    int len = 1;
+    while (true) {
+      const int k = len + l;  // does row r0 + k continue the run?
+      const bool on = off + k < page && r0 + k < a.rows && a.slots[min(r0 + k, a.rows - 1)] == slot + k;
+      const uint64_t stop = ~__ballot(on);
+      if (stop) {
+        len += __builtin_ctzll(stop);
+        break;
+      }
+      len += kWave;
+    }
+    const int id = slot >> a.shift;
+    if (len >= 8) {
+      append_run<D, kFp8, 2>(a, sh, w >> 1, w & 1, h, id, off, r0, len);
+    } else {
+      if ((turn & 1) == (w >> 1)) append_run<D, kFp8, 1>(a, sh, w & 1, 0, h, id, off, r0, len);
+      ++turn;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ attention
+//
+// Row i of request b stands at position past[b] + i and attends to positions
+// 0 .. past[b] + i: out = sum_j p_j v_j vs_j / sum_j p_j with p_j = e^(c ks_j
+// q . k_j - m). One pass over the keys with the running maximum m (in units
+// of log2) and sum in FP32. The scores are formed transposed (keys are the
+// products' rows, queries the columns), so that a lane's scores are
+// consecutive keys of one query and become the second operand of the value
+// product where they are, without a move between lanes: the rows of the key
+// operand are assigned to positions so that it comes out that way.
+//
+// A unit is 64 positions: four segments of 16, each within one page (pages
+// are multiples of 16 positions), so a segment has one key and value scale.
+constexpr int kUnit = 64;
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+struct Attend {
+  const uint16_t* q;
+  int64_t q_stride;  // elements between rows
+  const uint8_t* k;
+  const uint8_t* v;
+  const float* ks;
+  const float* vs;
+  const int* table;
+  const int* past;
+  const int* starts;
+  uint16_t* out;
+  float* part;     // [splits][rows][heads][D] of the narrow or wide splits
+  float2* part_ml;  // [splits][rows][heads]: maximum, sum
+  int* status;
+  int width, rows, kv, group, pages, shift, requests, max_rows;
+  int narrow_splits, wide_splits;
+  float scale;  // log2(e) * the softmax scale
+};
+
+__device__ __forceinline__ void raise(int* status, int bit) {
+  if (status != nullptr) atomicOr(status, bit);
+}
+
+// A request as the attention takes it.
+struct Request {
+  int row0, count, past;
+  int cap;   // positions that the table can hold
+  int len;   // positions that its last row sees, at most cap
+  bool narrow;
+};
+
+__device__ __forceinline__ bool request_at(const Attend& a, int b, Request& r) {
+  const int s0 = a.starts[b], s1 = a.starts[b + 1];
+  if (s1 == s0) return false;
+  if (s0 < 0 || s1 < s0 || s1 > a.rows || s1 - s0 > a.max_rows) {
+    if (threadIdx.x == 0) raise(a.status, kStatusRows);
+    return false;
+  }
+  r.row0 = s0;
+  r.count = s1 - s0;
+  r.past = a.past[b];
+  r.cap = clamp_int((int64_t)a.width << a.shift);
+  const int64_t len = (int64_t)r.past + r.count;
+  r.len = len < 0 ? 0 : len > r.cap ? r.cap : (int)len;
+  r.narrow = (int64_t)r.count * a.group <= 16;
+  if (len > r.cap && threadIdx.x == 0) raise(a.status, kStatusPage);
+  return true;
+}
+
+// The page of a request's segment that begins at position `at`, and whether
+// it may be read: a segment past the last position is not (its page number
+// may be anything), one whose number is outside the pool is not and `bad`.
+__device__ __forceinline__ int page_at(const Attend& a, const int* row, int at, int len, bool& bad) {
+  const int id = at < len ? row[at >> a.shift] : 0;
+  bad = (uint32_t)id >= (uint32_t)a.pages;
+  return bad ? 0 : id;
+}
+
+__device__ __forceinline__ float across_max16(float v) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+__device__ __forceinline__ float across_sum16(float v) {
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(y[0]) + __uint_as_float(y[1]);
+}
+__device__ __forceinline__ float across_max32(float v) {  // over lanes l, l ^ 32
+  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+__device__ __forceinline__ float across_sum32(float v) {
+  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(y[0]) + __uint_as_float(y[1]);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  bf16x2 r;
+  r[0] = (__bf16)a;
+  r[1] = (__bf16)b;
+  return __builtin_bit_cast(uint32_t, r);
+}
+
+template <bool kFp8>
+__device__ __forceinline__ bf16x8 codes8(uint32_t a, uint32_t b) {
+  uint4 r;
+  Code<kFp8>::pairs(a, r.x, r.y);
+  Code<kFp8>::pairs(b, r.z, r.w);
+  return __builtin_bit_cast(bf16x8, r);
+}
+
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The weight of a part whose maximum is m in a sum whose maximum is all: 0
+// for a part that saw nothing (m = -inf).
+__device__ __forceinline__ float part_weight(float m, float all) {
+  return m == -INFINITY ? 0.0f : exp2_of(m - all);
+}
+
+// ---- few columns: single tokens
+//
+// Up to 16 columns (rows x query heads of one KV head) of one request. Each
+// wave takes every fourth unit of the block's range and reads keys and values
+// from the cache straight into the operands' registers, the next unit's while
+// this one is computed: no LDS, no barrier until the waves' sums are joined.
+constexpr int kNarrowWaves = 4;
+
+template <int D>
+struct NarrowUnit {
+  uint4 k[4][D / 64];
+  uint4 v[D / 16];
+  float ks, vs;  // of this lane's segment, l / 16
+  bool bad;
+};
+
+template <int D>
+__device__ __forceinline__ void narrow_load(const Attend& a, const int* row, int h, int len, int u, NarrowUnit<D>& x) {
+  const int l = lane_id(), r = l & 15, g = l >> 4, page = 1 << a.shift;
+  bool bad_k;
+  const int at_k = u * kUnit + 16 * (r >> 2), at_v = u * kUnit + 16 * g;
+  const int id_k = page_at(a, row, at_k, len, bad_k), id_v = page_at(a, row, at_v, len, x.bad);
+  const uint8_t* k = a.k + ((((size_t)id_k * a.kv + h) << a.shift) + (at_k & (page - 1)) + (r & 3)) * D + g * (D / 4);
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) x.k[t][c] = *reinterpret_cast<const uint4*>(k + (size_t)(4 * t) * D + 16 * c);
+  const size_t head = (size_t)id_v * a.kv + h;
+  const uint8_t* v = a.v + ((head * D + r) << a.shift) + (at_v & (page - 1));
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) x.v[t] = *reinterpret_cast<const uint4*>(v + ((size_t)(16 * t) << a.shift));
+  x.ks = a.ks[head];
+  x.vs = a.vs[head];
+}
+
+template <int D>
+struct NarrowShared {
+  float m[kNarrowWaves][16], l[kNarrowWaves][16];
+  float o[kNarrowWaves][16][D + 4];
+};
+
+template <int D, bool kFp8>
+__global__ void __launch_bounds__(kNarrowWaves* kWave) k_kv8_attend_narrow(const Attend a) {
+  __shared__ NarrowShared<D> sh;
+  const int h = blockIdx.x % a.kv, sp = blockIdx.x / a.kv % a.narrow_splits, b = blockIdx.x / a.kv / a.narrow_splits;
+  Request rq;
+  if (!request_at(a, b, rq) || !rq.narrow) return;
+  const int units = (rq.len + kUnit - 1) / kUnit, per = (units + a.narrow_splits - 1) / a.narrow_splits;
+  const int u0 = sp * per, u1 = min(units, u0 + per);
+  if (sp > 0 && u0 >= u1) return;  // (the combination knows which parts there are)
+  const int w = wave_id(), l = lane_id(), r = l & 15, g = l >> 4;
+  const int* row = a.table + (size_t)b * a.width;
+  const int columns = rq.count * a.group;
+  // this lane's column: query row i, query head j of the KV head
+  const int ci = r / a.group, cj = r - ci * a.group;
+  const bool live = r < columns;
+  const int pos = live ? rq.past + ci : -1;
+  bf16x8 q[D / 32];
+  {
+    const uint16_t* src = a.q + (size_t)(rq.row0 + (live ? ci : 0)) * a.q_stride + (size_t)(h * a.group + (live ? cj : 0)) * D + g * (D / 4);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      Pack8 x = load8(src + 8 * c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x.w[i] = !live ? 0u : pos >= rq.cap ? 0x7fc07fc0u : x.w[i];  // past the table: NaN
+      q[c] = __builtin_bit_cast(bf16x8, x);
+    }
+  }
+  float m = -INFINITY, sum = 0.0f;
+  f32x4 o[D / 16];
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  NarrowUnit<D> next;
+  int u = u0 + w;
+  if (u < u1) narrow_load<D>(a, row, h, rq.len, u, next);
+  for (; u < u1; u += kNarrowWaves) {
+    NarrowUnit<D> x = next;
+    if (u + kNarrowWaves < u1) narrow_load<D>(a, row, h, rq.len, u + kNarrowWaves, next);
+    f32x4 s[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        const uint4 k = x.k[t][c / 2];
+        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(c & 1 ? codes8<kFp8>(k.z, k.w) : codes8<kFp8>(k.x, k.y), q[c], s[t], 0, 0, 0);
+      }
+    }
+    const int at = u * kUnit + 16 * g;  // this lane's first position
+    const bool whole = u * kUnit + kUnit - 1 <= rq.past && __ballot(x.bad) == 0;  // seen by every column
+    if (x.bad) {
+      raise(a.status, kStatusPage);
+      x.ks = __uint_as_float(0x7fc00000u);
+    }
+    const float ks = x.ks * a.scale;
+    if (!whole) {
+      // values behind the last position may be anything
+      const int left = x.bad ? 0 : rq.len - at;
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) {
+        uint32_t* const v = reinterpret_cast<uint32_t*>(&x.v[t]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int n = left - 4 * i;
+          v[i] &= n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (at + 4 * t + i > pos) s[t][i] = -INFINITY;
+    }
+    float most = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) most = fmaxf(most, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
+    // (a segment that the column sees nothing of has -inf here, whatever its scale)
+    most = across_max16(most == -INFINITY ? most : most * ks);
+    const float m_new = fmaxf(m, most), m_use = m_new == -INFINITY ? 0.0f : m_new;
+    if (__ballot(m_new != m) != 0) {
+      const float shrink = exp2_of(m - m_use);
+      sum *= shrink;
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) o[t] *= shrink;
+      m = m_new;
+    }
+    bf16x8 p[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      uint32_t pk[4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[i] = exp2_of(fmaf(s[2 * c + t][i], ks, -m_use));
+          if (!whole && at + 4 * (2 * c + t) + i > pos) e[i] = 0.0f;
+          sum += e[i];
+        }
+        // the probabilities' rounding to BF16, the value product's operand
+        // type: 2^-9 of each, independent of one another
+        float f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f[i] = e[i] * x.vs;
+          if (!whole && at + 4 * (2 * c + t) + i > pos) f[i] = 0.0f;  // (a scale may be NaN)
+        }
+        pk[2 * t] = pack_bf16(f[0], f[1]);
+        pk[2 * t + 1] = pack_bf16(f[2], f[3]);
+      }
+      p[c] = __builtin_bit_cast(bf16x8, uint4{pk[0], pk[1], pk[2], pk[3]});
+    }
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) {
+      o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes8<kFp8>(x.v[t].x, x.v[t].y), p[0], o[t], 0, 0, 0);
+      o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes8<kFp8>(x.v[t].z, x.v[t].w), p[1], o[t], 0, 0, 0);
+    }
+  }
+  // join the waves: o of this lane is column r, dimensions 16 t + 4 g + i
+  sum = across_sum16(sum);
+  if (g == 0) {
+    sh.m[w][r] = m;
+    sh.l[w][r] = sum;
+  }
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t)
+    *reinterpret_cast<f32x4*>(&sh.o[w][r][16 * t + 4 * g]) = o[t];
+  __syncthreads();
+  const int heads = a.kv * a.group;
+  for (int e = threadIdx.x; e < columns * (D / 4); e += kNarrowWaves * kWave) {
+    const int c = e / (D / 4), d = 4 * (e % (D / 4));
+    float all = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kNarrowWaves; ++i) all = fmaxf(all, sh.m[i][c]);
+    float total = 0.0f;
+    f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < kNarrowWaves; ++i) {
+      const float x = part_weight(sh.m[i][c], all);
+      total += x * sh.l[i][c];
+      acc += x * *reinterpret_cast<const f32x4*>(&sh.o[i][c][d]);
+    }
+    const int i = c / a.group, j = c - i * a.group;
+    const size_t at = (size_t)(rq.row0 + i) * heads + h * a.group + j;
+    if (a.narrow_splits == 1) {
+      const bool sees = rq.past + i >= 0;
+      uint2 y{0, 0};
+      if (sees) y = uint2{pack_bf16(acc[0] / total, acc[1] / total), pack_bf16(acc[2] / total, acc[3] / total)};
+      *reinterpret_cast<uint2*>(a.out + at * D + d) = y;
+    } else {
+      const size_t part = (size_t)sp * a.rows * heads + at;
+      *reinterpret_cast<f32x4*>(a.part + part * D + d) = acc;
+      if (d == 0) a.part_ml[part] = float2{all, total};
+    }
+  }
+}
+
+// ---- many columns: prompt chunks
+//
+// Tiles of 128 columns of one request and KV head, a wave for 32 of them
+// (v_mfma_f32_32x32x16_bf16); a unit's keys and values are converted to BF16
+// once for all four waves, in two LDS stages, the next unit's bytes loaded
+// while this one is computed.
+constexpr int kWideWaves = 4, kWideColumns = 32 * kWideWaves, kWideThreads = kWideWaves * kWave;
+
+template <int D>
+struct WideShared {
+  uint4 k[2][kUnit * (D / 8)];  // [position][dim], rows of D / 8 16-byte slots
+  uint4 v[2][D * (kUnit / 8)];  // [dim][position], scaled
+  float ks[2][4];               // the segments' key scales
+  int found[2];
+  int waves[kWideWaves];
+};
+
+// 16 rows read at one slot number spread over all 64 banks (two 128-byte rows
+// or one 256-byte row make a round of the banks).
+template <int kSlots>
+__device__ __forceinline__ int slot_of(int row, int c) {
+  return row * kSlots + (c ^ (kSlots == 8 ? (row >> 1) & 7 : row & 15));
+}
+
+template <int D>
+struct WideUnit {
+  uint4 k[D / 64], v[D / 64];
+  float ks, vs[D / 64];
+  uint32_t keep;  // positions of the segment to keep in v
+};
+
+// This thread's share: key position t / 4, 16 dimensions at 16 (t % 4) (and
+// 64 more); value dimension t / 4 (and + 64), segment t % 4.
+template <int D>
+__device__ __forceinline__ void wide_load(const Attend& a, const int* row, int h, int end, int u, WideUnit<D>& x) {
+  const int t = threadIdx.x, page = 1 << a.shift;
+  bool bad;
+  const int at_k = u * kUnit + t / 4;
+  const int id_k = page_at(a, row, at_k, end, bad);
+  const uint8_t* k = a.k + ((((size_t)id_k * a.kv + h) << a.shift) + (at_k & (page - 1))) * D + 16 * (t & 3);
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) x.k[c] = *reinterpret_cast<const uint4*>(k + 64 * c);
+  const int at_v = u * kUnit + 16 * (t & 3);
+  const int id_v = page_at(a, row, at_v, end, bad);
+  const size_t head = (size_t)id_v * a.kv + h;
+  const uint8_t* v = a.v + ((head * D + t / 4) << a.shift) + (at_v & (page - 1));
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) x.v[c] = *reinterpret_cast<const uint4*>(v + ((size_t)(64 * c) << a.shift));
+  x.ks = a.ks[head];
+  float vs = a.vs[head];
+  const int left = end - at_v;
+  x.keep = left >= 16 ? 0xffffu : left <= 0 ? 0u : (1u << left) - 1u;
+  // A page that cannot be read, or a value scale that is not finite, is NaN to
+  // the rows that attend to it and nothing to the others: the key scale
+  // carries it, since masked scores are replaced and masked values are not.
+  if (left <= 0) x.ks = vs = 0.0f;
+  else if (bad || !(fabsf(vs) < INFINITY)) x.ks = __uint_as_float(0x7fc00000u), vs = 0.0f, x.keep = 0u;
+  if (bad) raise(a.status, kStatusPage);
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) x.vs[c] = vs;
+}
+
+template <bool kFp8>
+__device__ __forceinline__ void scaled8(uint32_t a, uint32_t b, float scale, uint4& r) {
+  float f[4];
+  Code<kFp8>::values(a, f);
+  r.x = pack_bf16(f[0] * scale, f[1] * scale);
+  r.y = pack_bf16(f[2] * scale, f[3] * scale);
+  Code<kFp8>::values(b, f);
+  r.z = pack_bf16(f[0] * scale, f[1] * scale);
+  r.w = pack_bf16(f[2] * scale, f[3] * scale);
+}
+
+template <int D, bool kFp8>
+__device__ __forceinline__ void wide_store(WideShared<D>& sh, int stage, WideUnit<D>& x) {
+  const int t = threadIdx.x;
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) {
+    const int s = 8 * c + 2 * (t & 3);
+    uint4 lo, hi;
+    lo = __builtin_bit_cast(uint4, codes8<kFp8>(x.k[c].x, x.k[c].y));
+    hi = __builtin_bit_cast(uint4, codes8<kFp8>(x.k[c].z, x.k[c].w));
+    sh.k[stage][slot_of<D / 8>(t / 4, s)] = lo;
+    sh.k[stage][slot_of<D / 8>(t / 4, s + 1)] = hi;
+    if (x.keep != 0xffffu) {
+      uint32_t* const v = reinterpret_cast<uint32_t*>(&x.v[c]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t n = (x.keep >> (4 * i)) & 15u;  // 0, 1, 3, 7 or 15
+        v[i] &= n == 15u ? 0xffffffffu : n == 7u ? 0xffffffu : n == 3u ? 0xffffu : n == 1u ? 0xffu : 0u;
+      }
+    }
+    scaled8<kFp8>(x.v[c].x, x.v[c].y, x.vs[c], lo);
+    scaled8<kFp8>(x.v[c].z, x.v[c].w, x.vs[c], hi);
+    sh.v[stage][slot_of<8>(t / 4 + 64 * c, 2 * (t & 3))] = lo;
+    sh.v[stage][slot_of<8>(t / 4 + 64 * c, 2 * (t & 3) + 1)] = hi;
+  }
+  if (t < 4) sh.ks[stage][t] = x.ks;
+}
+
+template <int D, bool kFp8>
+__global__ void __launch_bounds__(kWideThreads) k_kv8_attend_wide(const Attend a) {
+  __shared__ WideShared<D> sh;
+  const int h = blockIdx.x % a.kv, sp = blockIdx.x / a.kv % a.wide_splits, tile = blockIdx.x / a.kv / a.wide_splits;
+  const int w = wave_id(), l = lane_id();
+  // the request of this tile: the wide requests' tiles in order
+  {
+    const int each = (a.requests + kWideThreads - 1) / kWideThreads, b0 = threadIdx.x * each;
+    const auto tiles_of = [&](int b) {
+      if (b >= a.requests) return 0;
+      const int s0 = a.starts[b], s1 = a.starts[b + 1];
+      if (s0 < 0 || s1 <= s0 || s1 > a.rows || s1 - s0 > a.max_rows || (int64_t)(s1 - s0) * a.group <= 16) return 0;
+      return (int)(((int64_t)(s1 - s0) * a.group + kWideColumns - 1) / kWideColumns);
+    };
+    int mine = 0;
+    for (int j = 0; j < each; ++j) mine += tiles_of(b0 + j);
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int x = __shfl_up(upto, d, kWave);
+      if (l >= d) upto += x;
+    }
+    if (l == kWave - 1) sh.waves[w] = upto;
+    if (threadIdx.x == 0) sh.found[0] = -1;
+    __syncthreads();
+    for (int i = 0; i < w; ++i) upto += sh.waves[i];
+    int first = upto - mine;
+    if (tile >= first && tile < upto) {
+      for (int j = 0; j < each; ++j) {
+        const int n = tiles_of(b0 + j);
+        if (tile >= first && tile < first + n) {
+          sh.found[0] = b0 + j;
+          sh.found[1] = n - 1 - (tile - first);  // the longest first
+        }
+        first += n;
+      }
+    }
+    __syncthreads();
+  }
+  const int b = sh.found[0];
+  if (b < 0) return;
+  Request rq;
+  if (!request_at(a, b, rq)) return;
+  const int* row = a.table + (size_t)b * a.width;
+  const int columns = rq.count * a.group, c0 = sh.found[1] * kWideColumns;
+  const int last = (min(c0 + kWideColumns, columns) - 1) / a.group;  // the tile's last query row
+  const int64_t end64 = (int64_t)rq.past + last + 1;
+  const int end = end64 < 0 ? 0 : end64 > rq.cap ? rq.cap : (int)end64;
+  const int units = (rq.len + kUnit - 1) / kUnit, per = (units + a.wide_splits - 1) / a.wide_splits;
+  const int u0 = sp * per, u1 = min((end + kUnit - 1) / kUnit, u0 + per);
+  if (sp > 0 && u0 >= u1) return;
+  const int half = l >> 5;
+  const int column = c0 + 32 * w + (l & 31);
+  const bool live = column < columns;
+  const int ci = live ? column / a.group : 0, cj = live ? column - ci * a.group : 0;
+  const int pos = live ? rq.past + ci : -1;
+  bf16x8 q[D / 16];
+  {
+    const uint16_t* src = a.q + (size_t)(rq.row0 + ci) * a.q_stride + (size_t)(h * a.group + cj) * D + 8 * half;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      Pack8 x = load8(src + 16 * c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x.w[i] = !live ? 0u : pos >= rq.cap ? 0x7fc07fc0u : x.w[i];
+      q[c] = __builtin_bit_cast(bf16x8, x);
+    }
+  }
+  float m = -INFINITY, sum = 0.0f;
+  f32x16 o[D / 32];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+  // the first position that some column of this wave does not see, and the
+  // last that one does
+  const int wave_first = rq.past + min((c0 + 32 * w) / a.group, rq.count - 1);
+  const int wave_last = rq.past + min((c0 + 32 * w + 31) / a.group, rq.count - 1);
+  const bool wave_live = c0 + 32 * w < columns;
+  // operand row l % 32 of a key tile is position rho with bits 2 and 3
+  // exchanged: the results of lane half `half`, i = 0 .. 15, are then
+  // positions 16 (i / 8) + 8 half + i % 8
+  const int rho = (l & 0x13) | ((l & 4) << 1) | ((l & 8) >> 1);
+  WideUnit<D> next;
+  if (u0 < u1) {
+    wide_load<D>(a, row, h, end, u0, next);
+    wide_store<D, kFp8>(sh, 0, next);
+  }
+  __syncthreads();
+  for (int u = u0; u < u1; ++u) {
+    const int stage = (u - u0) & 1;
+    if (u + 1 < u1) wide_load<D>(a, row, h, end, u + 1, next);
+    if (wave_live && u * kUnit <= wave_last) {
+      f32x16 s[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          const bf16x8 k = __builtin_bit_cast(bf16x8, sh.k[stage][slot_of<D / 8>(32 * t + rho, 2 * c + half)]);
+          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[c], s[t], 0, 0, 0);
+        }
+      }
+      float ks[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ks[i] = sh.ks[stage][i] * a.scale;
+      const int at = u * kUnit + 8 * half;
+      const bool whole = u * kUnit + kUnit - 1 <= wave_first;
+      if (!whole) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (at + 32 * t + 16 * (i / 8) + i % 8 > pos) s[t][i] = -INFINITY;
+      }
+      float most = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = s[t][8 * e];
+#pragma unroll
+          for (int i = 1; i < 8; ++i) x = fmaxf(x, s[t][8 * e + i]);
+          most = fmaxf(most, x == -INFINITY ? x : x * ks[2 * t + e]);
+        }
+      most = across_max32(most);
+      const float m_new = fmaxf(m, most), m_use = m_new == -INFINITY ? 0.0f : m_new;
+      if (__ballot(m_new != m) != 0) {
+        const float shrink = exp2_of(m - m_use);
+        sum *= shrink;
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t) o[t] *= shrink;
+        m = m_new;
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            f[i] = exp2_of(fmaf(s[t][8 * e + i], ks[2 * t + e], -m_use));
+            if (!whole && at + 32 * t + 16 * e + i > pos) f[i] = 0.0f;
+            sum += f[i];
+          }
+          const bf16x8 p = __builtin_bit_cast(
+              bf16x8, uint4{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])});
+#pragma unroll
+          for (int d = 0; d < D / 32; ++d) {
+            const bf16x8 v = __builtin_bit_cast(bf16x8, sh.v[stage][slot_of<8>(32 * d + (l & 31), 4 * t + 2 * e + half)]);
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, p, o[d], 0, 0, 0);
+          }
+        }
+    }
+    if (u + 1 < u1) wide_store<D, kFp8>(sh, stage ^ 1, next);
+    __syncthreads();
+  }
+  if (!live) return;
+  sum = across_sum32(sum);
+  const int heads = a.kv * a.group;
+  const size_t at = (size_t)(rq.row0 + ci) * heads + h * a.group + cj;
+  const size_t part = (size_t)sp * a.rows * heads + at;
+  const float inv = 1.0f / sum;
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = 32 * t + 8 * i + 4 * half;
+      const f32x4 x{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
+      if (a.wide_splits == 1) {
+        uint2 y{0, 0};
+        if (pos >= 0) y = uint2{pack_bf16(x[0] * inv, x[1] * inv), pack_bf16(x[2] * inv, x[3] * inv)};
+        *reinterpret_cast<uint2*>(a.out + at * D + d) = y;
+      } else {
+        *reinterpret_cast<f32x4*>(a.part + part * D + d) = x;
+      }
+    }
+  if (a.wide_splits > 1 && half == 0) a.part_ml[part] = float2{m, sum};
+}
+
+// ---- the parts of a split range of keys joined, in the parts' order: a wave
+// for one row and query head.
+constexpr int kCombineWaves = 4;
+
+// The request that row x belongs to (requests if it is behind the last), by
+// one wave: 64 of the offsets at a time.
+__device__ __forceinline__ int request_of_row(const int* starts, int n, int x) {
+  const int l = lane_id(), step = (n + kWave) / kWave;  // step * 64 > n
+  const int at = l * step;
+  const int coarse = __popcll(__ballot(at <= n && starts[min(at, n)] <= x)) - 1;
+  if (coarse < 0) return n;
+  int found = coarse * step;
+  for (int i0 = 1; i0 < step; i0 += kWave) {
+    const int i = coarse * step + i0 + l;
+    found += __popcll(__ballot(i0 + l < step && i <= n && starts[min(i, n)] <= x));
+  }
+  return found;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kCombineWaves* kWave) k_kv8_combine(const Attend a) {
+  const int heads = a.kv * a.group, l = lane_id();
+  const int64_t item = (int64_t)blockIdx.x * kCombineWaves + wave_id();
+  if (item >= (int64_t)a.rows * heads) return;
+  const int x = (int)(item / heads);
+  const int b = __builtin_amdgcn_readfirstlane(request_of_row(a.starts, a.requests, x));
+  if (b >= a.requests) return;
+  Request rq;
+  if (!request_at(a, b, rq)) return;
+  const int splits = rq.narrow ? a.narrow_splits : a.wide_splits;
+  if (splits == 1) return;
+  const int64_t pos = (int64_t)rq.past + (x - rq.row0);
+  const int units = (rq.len + kUnit - 1) / kUnit, per = (units + splits - 1) / splits;
+  const int seen = (int)((min(pos + 1, (int64_t)rq.len) + kUnit - 1) / kUnit);  // units that the row sees
+  const int parts = pos < 0 ? 0 : (seen + per - 1) / per;                      // 1 .. splits, at most 64
+  const size_t stride = (size_t)a.rows * heads;
+  float2 ml{-INFINITY, 0.0f};
+  if (l < parts) ml = a.part_ml[l * stride + item];
+  const float all = wave_max(ml.x);
+  const float weight = part_weight(ml.x, all);
+  const float total = wave_sum(weight * ml.y);
+  float acc[D / 64] = {};
+  for (int i = 0; i < parts; ++i) {
+    const float x_i = lane_value(weight, i);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) acc[c] += x_i * a.part[(i * stride + item) * D + 64 * c + l];
+  }
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c)
+    a.out[item * D + 64 * c + l] = pos < 0 ? (uint16_t)0 : f32_to_bf16(acc[c] / total);
+}
+
+// ------------------------------------------------------------------ host
+
+int page_shift(int32_t page) {
+  for (int s = 4; s <= 8; ++s)
+    if (page == 1 << s) return s;
+  return -1;
+}
+
+bool cache_shape(int32_t pages, int32_t page, int32_t kv, int32_t dim, int32_t format) {
+  if (page_shift(page) < 0) return set_error(LFM25_EINVAL, "page must be 16, 32, 64, 128 or 256"), false;
+  if (pages < 1 || (int64_t)pages * page > INT32_MAX) return set_error(LFM25_EINVAL, "pages * page must be in [1, 2^31)"), false;
+  if (kv < 1 || kv > 256) return set_error(LFM25_EINVAL, "kv_heads must be in [1, 256]"), false;
+  if (dim != 64 && dim != 128) return set_error(LFM25_EINVAL, "head_dim must be 64 or 128"), false;
+  if (format != LFM25_KV8_INT8 && format != LFM25_KV8_FP8) return set_error(LFM25_EINVAL, "unknown 8-bit format %d", format), false;
+  return true;
+}
+
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
+
+struct Splits {
+  int narrow, wide;     // parts of a request's keys for each kind of request
+  int64_t wide_tiles;   // most tiles that the rows can make
+  bool has_wide;
+};
+
+// Parts: enough blocks to fill the chip (256 CUs, four narrow blocks or two
+// wide ones each) where the requests alone do not, of at least 256 (narrow:
+// a unit per wave) and 512 positions, from what the host knows: the lengths
+// are on the device, the table's width bounds them.
+Splits splits_for(int32_t rows, int32_t requests, int32_t kv, int32_t group, int32_t max_rows, int32_t width, int32_t page) {
+  Splits s{1, 1, 0, false};
+  const int64_t positions = std::min<int64_t>((int64_t)width * page, INT32_MAX);
+  const auto parts = [&](int64_t blocks, int64_t wanted, int64_t least) {
+    const int64_t p = std::min((wanted + blocks - 1) / blocks, positions / least);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(p, kWave));
+  };
+  s.narrow = parts((int64_t)std::min(requests, rows) * kv, 1024, 256);
+  s.has_wide = (int64_t)max_rows * group > 16;
+  if (s.has_wide) {
+    const int64_t columns = (int64_t)rows * group;
+    s.wide_tiles = columns / kWideColumns + std::min<int64_t>(requests, columns / 17 + 1);
+    s.wide = parts(s.wide_tiles * kv, 512, 512);
+  }
+  return s;
+}
+
+size_t part_floats(const Splits& s, int64_t rows, int64_t heads, int64_t dim) {
+  const int most = std::max(s.narrow, s.wide);
+  return most == 1 ? 0 : (size_t)(most * rows * heads * (dim + 2));
+}
+
+template <int D, bool kFp8>
+int attend(const Attend& a, const Splits& s, hipStream_t stream) {
+  const int64_t narrow = (int64_t)a.requests * a.kv * a.narrow_splits, wide = s.wide_tiles * a.kv * a.wide_splits;
+  hipLaunchKernelGGL((k_kv8_attend_narrow<D, kFp8>), dim3((unsigned)narrow), dim3(kNarrowWaves * kWave), 0, stream, a);
+  if (s.has_wide)
+    hipLaunchKernelGGL((k_kv8_attend_wide<D, kFp8>), dim3((unsigned)wide), dim3(kWideThreads), 0, stream, a);
+  if (a.narrow_splits > 1 || a.wide_splits > 1) {
+    const int64_t items = (int64_t)a.rows * a.kv * a.group;
+    hipLaunchKernelGGL((k_kv8_combine<D>), dim3((unsigned)((items + kCombineWaves - 1) / kCombineWaves)),
+                       dim3(kCombineWaves * kWave), 0, stream, a);
+  }
+  return check_launch("lfm25_kv8_attention");
+}
+
+}  // namespace
+}  // namespace lfm25
+
+using namespace lfm25;
+
+extern "C" int lfm25_kv8_plan(const int32_t* past, const int32_t* counts, int32_t requests, int32_t* block_table, int32_t width,
+                              int32_t* free_pages, int32_t ring, const int64_t* cursor, int32_t* row_starts, int32_t* slots,
+                              int32_t rows, int64_t* next_cursor, int32_t* status, int32_t page, lfm25_stream_t stream) {
+  LFM25_REQUIRE(past && counts && block_table && free_pages && cursor && row_starts && slots && next_cursor && status,
+                "lfm25_kv8_plan: null pointer");
+  LFM25_REQUIRE(page_shift(page) >= 0, "lfm25_kv8_plan: page must be 16, 32, 64, 128 or 256");
+  LFM25_REQUIRE(requests >= 1 && requests <= kMaxRequests, "lfm25_kv8_plan: requests must be in [1, %d]", kMaxRequests);
+  LFM25_REQUIRE(width >= 1 && (int64_t)width * page <= INT32_MAX, "lfm25_kv8_plan: width * page must be in [1, 2^31)");
+  LFM25_REQUIRE(ring >= 1 && rows >= 1, "lfm25_kv8_plan: an empty ring or no rows");
+  LFM25_REQUIRE(aligned4(past) && aligned4(counts) && aligned4(block_table) && aligned4(free_pages) && aligned4(row_starts) &&
+                    aligned4(slots) && aligned4(status) && aligned8(cursor) && aligned8(next_cursor),
+                "lfm25_kv8_plan: misaligned pointer");
+  hipLaunchKernelGGL(k_kv8_plan, dim3(1), dim3(kPlanThreads), 0, stream, past, counts, requests, block_table, width, free_pages, ring,
+                     cursor, row_starts, slots, rows, next_cursor, status, page_shift(page));
+  return check_launch("lfm25_kv8_plan");
+}
+
+extern "C" int lfm25_kv8_append(const uint16_t* keys, int64_t key_stride, const uint16_t* values, int64_t value_stride,
+                                const int32_t* slots, int32_t rows, void* key_cache, void* value_cache, float* key_scales,
+                                float* value_scales, int32_t pages, int32_t page, int32_t kv_heads, int32_t head_dim,
+                                int32_t format, lfm25_stream_t stream) {
+  LFM25_REQUIRE(keys && values && slots && key_cache && value_cache && key_scales && value_scales, "lfm25_kv8_append: null pointer");
+  if (!cache_shape(pages, page, kv_heads, head_dim, format)) return LFM25_EINVAL;
+  LFM25_REQUIRE(rows >= 1, "lfm25_kv8_append: no rows");
+  const int64_t row = (int64_t)kv_heads * head_dim;
+  LFM25_REQUIRE(key_stride >= row && value_stride >= row && key_stride % 8 == 0 && value_stride % 8 == 0,
+                "lfm25_kv8_append: row strides must be multiples of 8 of at least kv_heads * head_dim");
+  LFM25_REQUIRE(aligned16(keys) && aligned16(values) && aligned16(key_cache) && aligned16(value_cache),
+                "lfm25_kv8_append: keys, values and caches must be 16-byte aligned");
+  LFM25_REQUIRE(aligned4(slots) && aligned4(key_scales) && aligned4(value_scales), "lfm25_kv8_append: misaligned pointer");
+  Append a{};
+  a.x[0] = keys, a.x[1] = values;
+  a.stride[0] = key_stride, a.stride[1] = value_stride;
+  a.cache[0] = static_cast<uint8_t*>(key_cache), a.cache[1] = static_cast<uint8_t*>(value_cache);
+  a.scales[0] = key_scales, a.scales[1] = value_scales;
+  a.slots = slots;
+  a.rows = rows, a.kv = kv_heads, a.pages = pages, a.shift = page_shift(page);
+  a.chunk = rows <= 512 ? 2 : 8;
+  const dim3 grid((unsigned)((rows + a.chunk - 1) / a.chunk), (unsigned)kv_heads), block(kAppendThreads);
+  if (head_dim == 64) {
+    if (format == LFM25_KV8_FP8) hipLaunchKernelGGL((k_kv8_append<64, true>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((k_kv8_append<64, false>), grid, block, 0, stream, a);
+  } else {
+    if (format == LFM25_KV8_FP8) hipLaunchKernelGGL((k_kv8_append<128, true>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((k_kv8_append<128, false>), grid, block, 0, stream, a);
+  }
+  return check_launch("lfm25_kv8_append");
+}
+
+static bool attend_shape(int32_t rows, int32_t heads, int32_t kv_heads, int32_t requests, int32_t max_rows, int32_t width, int32_t page) {
+  if (kv_heads < 1 || heads < 1 || heads % kv_heads != 0 || heads / kv_heads > 16)
+    return set_error(LFM25_EINVAL, "heads must be a multiple of kv_heads, at most 16 times it"), false;
+  if (rows < 1 || (int64_t)rows * heads > INT32_MAX) return set_error(LFM25_EINVAL, "rows * heads must be in [1, 2^31)"), false;
+  if (requests < 1 || requests > kMaxRequests) return set_error(LFM25_EINVAL, "requests must be in [1, %d]", kMaxRequests), false;
+  if (max_rows < 1) return set_error(LFM25_EINVAL, "max_rows must be positive"), false;
+  if (width < 1 || (int64_t)width * page > INT32_MAX) return set_error(LFM25_EINVAL, "width * page must be in [1, 2^31)"), false;
+  return true;
+}
+
+extern "C" size_t lfm25_kv8_attention_workspace_bytes(int32_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                                      int32_t requests, int32_t max_rows, int32_t width, int32_t page) {
+  if (page_shift(page) < 0 || (head_dim != 64 && head_dim != 128) ||
+      !attend_shape(rows, heads, kv_heads, requests, max_rows, width, page))
+    return 0;
+  const Splits s = splits_for(rows, requests, kv_heads, heads / kv_heads, std::min(max_rows, rows), width, page);
+  return 4 * part_floats(s, rows, heads, head_dim);
+}
+
+extern "C" int lfm25_kv8_attention(const uint16_t* query, int64_t query_stride, const void* key_cache, const void* value_cache,
+                                   const float* key_scales, const float* value_scales, const int32_t* block_table, int32_t width,
+                                   const int32_t* past, const int32_t* row_starts, int32_t requests, uint16_t* output, int32_t rows,
+                                   int32_t heads, int32_t max_rows, float scale, int32_t pages, int32_t page, int32_t kv_heads,
+                                   int32_t head_dim, int32_t format, int32_t* status, void* workspace, lfm25_stream_t stream) {
+  LFM25_REQUIRE(query && key_cache && value_cache && key_scales && value_scales && block_table && past && row_starts && output,
+                "lfm25_kv8_attention: null pointer");
+  if (!cache_shape(pages, page, kv_heads, head_dim, format)) return LFM25_EINVAL;
+  if (!attend_shape(rows, heads, kv_heads, requests, max_rows, width, page)) return LFM25_EINVAL;
+  LFM25_REQUIRE(query_stride >= (int64_t)heads * head_dim && query_stride % 8 == 0,
+                "lfm25_kv8_attention: the query's row stride must be a multiple of 8 of at least heads * head_dim");
+  LFM25_REQUIRE(aligned16(query) && aligned16(key_cache) && aligned16(value_cache) && aligned16(output),
+                "lfm25_kv8_attention: query, output and caches must be 16-byte aligned");
+  LFM25_REQUIRE(aligned4(key_scales) && aligned4(value_scales) && aligned4(block_table) && aligned4(past) && aligned4(row_starts) &&
+                    aligned4(status),
+                "lfm25_kv8_attention: misaligned pointer");
+  LFM25_REQUIRE(std::isfinite(scale) && scale >= 0.0f, "lfm25_kv8_attention: scale must be finite and not negative");
+  max_rows = std::min(max_rows, rows);
+  const Splits s = splits_for(rows, requests, kv_heads, heads / kv_heads, max_rows, width, page);
+  const size_t floats = part_floats(s, rows, heads, head_dim);
+  LFM25_REQUIRE(floats == 0 || (workspace != nullptr && aligned16(workspace)),
+                "lfm25_kv8_attention: needs a 16-byte aligned workspace of lfm25_kv8_attention_workspace_bytes()");
+  Attend a{};
+  a.q = query, a.q_stride = query_stride;
+  a.k = static_cast<const uint8_t*>(key_cache), a.v = static_cast<const uint8_t*>(value_cache);
+  a.ks = key_scales, a.vs = value_scales;
+  a.table = block_table, a.past = past, a.starts = row_starts;
+  a.out = output;
+  a.part = static_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)std::max(s.narrow, s.wide) * rows * heads * head_dim);
+  a.status = status;
+  a.width = width, a.rows = rows, a.kv = kv_heads, a.group = heads / kv_heads, a.pages = pages, a.shift = page_shift(page);
+  a.requests = requests, a.max_rows = max_rows;
+  a.narrow_splits = s.narrow, a.wide_splits = s.wide;
+  a.scale = scale * 1.4426950408889634f;
+  if (head_dim == 64) return format == LFM25_KV8_FP8 ? attend<64, true>(a, s, stream) : attend<64, false>(a, s, stream);
+  return format == LFM25_KV8_FP8 ? attend<128, true>(a, s, stream) : attend<128, false>(a, s, stream);
+}

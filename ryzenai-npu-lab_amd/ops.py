@@ -533,3 +533,161 @@ def bf16_f32_matmul(input0, input1, output, *, M: int, K: int, N: int, n_cores: 
         raise ValueError("Weight reuse probe requires M=48")
     _lib.call("lfm25_bf16_f32_matmul", _bf(input0, "input0", M * K), _bf(input1, "input1", K * N),
               _f32(output, "output", M * N), M, K, N, _stream())
+
+
+# ---------------------------------------------------------------- paged 8-bit KV cache
+#
+# A pool of pages of `page` positions in int8 or FP8 (e4m3), one FP32 scale
+# per page and KV head; block tables give each request's pages. A pass is
+# kv8_plan, then per layer kv8_append and kv8_attention (lfm25_kv8_* in
+# include/lfm25_hip.h has the definitions). Nothing here waits for the GPU,
+# and all of it may be captured into a graph.
+
+KV8_LENGTH, KV8_TABLE, KV8_POOL, KV8_ROWS = 1, 2, 4, 8  # kv8_plan's status
+KV8_BAD_PAGE, KV8_BAD_ROWS = 1, 2                       # kv8_attention's status bits
+_KV8_FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
+_KV8_PAGES = (16, 32, 64, 128, 256)
+
+
+def _here(*tensors) -> None:
+    """All on the current device, whose stream the call goes to."""
+    device = torch.cuda.current_device()
+    for t in tensors:
+        if t.get_device() != device:
+            raise ValueError(f"tensors must be on the current device (cuda:{device}), got {t.device}")
+
+
+def _kv8_rows(t, name: str, heads: int, dim: int, rows: int) -> int:
+    """Address of BF16 rows [rows, heads, dim] whose rows may be apart."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a GPU tensor")
+    if t.dtype != torch.bfloat16:
+        raise ValueError(f"{name} must be {torch.bfloat16}, got {t.dtype}")
+    if t.shape != (rows, heads, dim):
+        raise ValueError(f"{name} must be [{rows}, {heads}, {dim}], got {list(t.shape)}")
+    s = t.stride()
+    if s[2] != 1 or (heads > 1 and s[1] != dim):
+        raise ValueError(f"{name}: a row's heads must be contiguous")
+    return t.data_ptr()
+
+
+def _kv8_stride(t) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _kv8_cache(key_cache, value_cache, key_scales, value_scales):
+    """(pages, page, kv_heads, dim, format) of a cache's four tensors."""
+    if not isinstance(key_cache, torch.Tensor) or key_cache.dim() != 4:
+        raise ValueError("key_cache must be [pages, kv_heads, page, dim]")
+    form = _KV8_FORMATS.get(key_cache.dtype)
+    if form is None:
+        raise ValueError(f"key_cache must be torch.int8 or torch.float8_e4m3fn, got {key_cache.dtype}")
+    pages, kv, page, dim = key_cache.shape
+    if page not in _KV8_PAGES or dim not in (64, 128):
+        raise ValueError(f"pages must be of 16, 32, 64, 128 or 256 positions and dim 64 or 128, got {page} and {dim}")
+    _check(key_cache, "key_cache", key_cache.dtype)
+    _check(value_cache, "value_cache", key_cache.dtype)
+    if value_cache.shape != (pages, kv, dim, page):
+        raise ValueError(f"value_cache must be [{pages}, {kv}, {dim}, {page}], got {list(value_cache.shape)}")
+    for t, name in ((key_scales, "key_scales"), (value_scales, "value_scales")):
+        _f32(t, name)
+        if t.shape != (pages, kv):
+            raise ValueError(f"{name} must be [{pages}, {kv}], got {list(t.shape)}")
+    return pages, page, kv, dim, form
+
+
+def kv8_plan(past, counts, block_table, free_pages, cursor, row_starts, slots, next_cursor, status, *, page: int) -> None:
+    """Pages, row offsets and cache slots of a pass from the requests' lengths
+    (lfm25_kv8_plan). past, counts: int32 [requests], positions held and new
+    rows (counts[b] < 0 ends request b and gives its pages back). block_table:
+    int32 [requests, width], extended in place. free_pages: int32 [ring], a
+    ring of free page numbers, of which the entries cursor[0] .. cursor[1]
+    (int64, counted on without end) are free. Written: row_starts int32
+    [requests + 1], slots int32 [rows] (-1: a refused request's row, or behind
+    the last), next_cursor int64 [2] (may be cursor), status int32 [requests]
+    (0, or KV8_LENGTH / KV8_TABLE / KV8_POOL / KV8_ROWS)."""
+    if page not in _KV8_PAGES:
+        raise ValueError("page must be 16, 32, 64, 128 or 256")
+    n = past.numel() if isinstance(past, torch.Tensor) else 0
+    if not 1 <= n <= 4096:
+        raise ValueError("past must be a tensor of 1 to 4096 lengths")
+    _i32(past, "past")
+    _i32(counts, "counts", n)
+    _i32(block_table, "block_table")
+    if block_table.dim() != 2 or block_table.shape[0] != n or block_table.shape[1] < 1:
+        raise ValueError(f"block_table must be [{n}, width]")
+    _i32(free_pages, "free_pages")
+    _check(cursor, "cursor", torch.int64, 2)
+    _i32(row_starts, "row_starts", n + 1)
+    _i32(slots, "slots")
+    _check(next_cursor, "next_cursor", torch.int64, 2)
+    _i32(status, "status", n)
+    if free_pages.numel() < 1 or slots.numel() < 1:
+        raise ValueError("free_pages and slots must not be empty")
+    _here(past, counts, block_table, free_pages, cursor, row_starts, slots, next_cursor, status)
+    _lib.call("lfm25_kv8_plan", past.data_ptr(), counts.data_ptr(), n, block_table.data_ptr(), block_table.shape[1],
+              free_pages.data_ptr(), free_pages.numel(), cursor.data_ptr(), row_starts.data_ptr(), slots.data_ptr(),
+              slots.numel(), next_cursor.data_ptr(), status.data_ptr(), page, _stream())
+
+
+def kv8_append(keys, values, slots, key_cache, value_cache, key_scales, value_scales) -> None:
+    """New keys and values into the 8-bit cache (lfm25_kv8_append). keys,
+    values: BF16 [rows, kv_heads, dim], rows may be strided (slices of a fused
+    q | k | v product). slots: int32 [rows] as kv8_plan gives them (-1 leaves a
+    row out). Written in place: key_cache [pages, kv_heads, page, dim] and
+    value_cache [pages, kv_heads, dim, page] in torch.int8 or
+    torch.float8_e4m3fn, key_scales and value_scales FP32 [pages, kv_heads]."""
+    pages, page, kv, dim, form = _kv8_cache(key_cache, value_cache, key_scales, value_scales)
+    _i32(slots, "slots")
+    rows = slots.numel()
+    k, v = _kv8_rows(keys, "keys", kv, dim, rows), _kv8_rows(values, "values", kv, dim, rows)
+    if rows == 0:
+        return
+    _here(keys, values, slots, key_cache, value_cache, key_scales, value_scales)
+    _lib.call("lfm25_kv8_append", k, _kv8_stride(keys), v, _kv8_stride(values), slots.data_ptr(), rows, key_cache.data_ptr(),
+              value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), pages, page, kv, dim, form, _stream())
+
+
+def kv8_attention(query, key_cache, value_cache, key_scales, value_scales, block_table, past, row_starts, output, *,
+                  max_rows: int, scale: float | None = None, status=None) -> None:
+    """Causal attention of a pass's rows over the 8-bit cache
+    (lfm25_kv8_attention). query: BF16 [rows, heads, dim], rows may be strided;
+    heads a multiple (up to 16) of the cache's kv_heads. block_table int32
+    [requests, width], past int32 [requests], row_starts int32 [requests + 1]:
+    row i of request b stands at position past[b] + i and sees the positions up
+    to it, which kv8_append has written. max_rows: the most rows of one
+    request. scale: of the scores, 1 / sqrt(dim) by default. Written: output
+    BF16 [rows, heads, dim], contiguous; status (int32 [1], optional) gets bits
+    KV8_BAD_PAGE / KV8_BAD_ROWS set."""
+    pages, page, kv, dim, form = _kv8_cache(key_cache, value_cache, key_scales, value_scales)
+    _bf(output, "output")
+    if output.dim() != 3 or output.shape[2] != dim or output.shape[1] % kv or not 1 <= output.shape[1] // kv <= 16:
+        raise ValueError(f"output must be [rows, heads, {dim}] with heads a multiple (1 to 16) of {kv}")
+    rows, heads = output.shape[:2]
+    q = _kv8_rows(query, "query", heads, dim, rows)
+    _i32(past, "past")
+    n = past.numel()
+    if not 1 <= n <= 4096:
+        raise ValueError("past must hold 1 to 4096 lengths")
+    _i32(row_starts, "row_starts", n + 1)
+    _i32(block_table, "block_table")
+    if block_table.dim() != 2 or block_table.shape[0] != n or block_table.shape[1] < 1:
+        raise ValueError(f"block_table must be [{n}, width]")
+    if max_rows < 1:
+        raise ValueError("max_rows must be positive")
+    scale = dim ** -0.5 if scale is None else scale
+    if not 0.0 <= scale < float("inf"):
+        raise ValueError("scale must be finite and not negative")
+    flags = 0 if status is None else _i32(status, "status", 1)
+    if rows == 0:
+        return
+    _here(query, key_cache, value_cache, key_scales, value_scales, block_table, past, row_starts, output,
+          *(() if status is None else (status,)))
+    width = block_table.shape[1]
+    max_rows = min(max_rows, rows)
+    need = _lib.load().lfm25_kv8_attention_workspace_bytes(rows, heads, kv, dim, n, max_rows, width, page)
+    ws = torch.empty(need, dtype=torch.uint8, device=output.device) if need else None
+    _lib.call("lfm25_kv8_attention", q, _kv8_stride(query), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
+              value_scales.data_ptr(), block_table.data_ptr(), width, past.data_ptr(), row_starts.data_ptr(), n,
+              output.data_ptr(), rows, heads, max_rows, scale, pages, page, kv, dim, form, flags,
+              ws.data_ptr() if need else 0, _stream())
