@@ -435,8 +435,14 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv8_append(const Append a) {
 //
 // A unit is 64 positions: four segments of 16, each within one page (pages
 // are multiples of 16 positions), so a segment has one key and value scale.
+// Neither costs an operation per score: the key scale is the factor of the
+// exponent's one fused multiply-add, the value scale (less the largest seen,
+// so that no sum passes the range of the values) its addend as a logarithm,
+// and the sum of the probabilities takes that factor back out as the other
+// operand of its dot product.
 constexpr int kUnit = 64;
 
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -452,11 +458,11 @@ struct Attend {
   const int* past;
   const int* starts;
   uint16_t* out;
-  float* part;     // [splits][rows][heads][D] of the narrow or wide splits
+  float* part;      // [splits][rows][heads][D], each part's own result
   float2* part_ml;  // [splits][rows][heads]: maximum, sum
   int* status;
   int width, rows, kv, group, pages, shift, requests, max_rows;
-  int narrow_splits, wide_splits;
+  int narrow_splits, wide_splits, wide_blocks;
   float scale;  // log2(e) * the softmax scale
 };
 
@@ -467,13 +473,14 @@ __device__ __forceinline__ void raise(int* status, int bit) {
 // A request as the attention takes it.
 struct Request {
   int row0, count, past;
-  int cap;   // positions that the table can hold
-  int len;   // positions that its last row sees, at most cap
+  int cap;  // positions that the table can hold
+  int len;  // positions that its last row sees, at most cap
   bool narrow;
 };
 
 __device__ __forceinline__ bool request_at(const Attend& a, int b, Request& r) {
   const int s0 = a.starts[b], s1 = a.starts[b + 1];
+  r.past = a.past[b];
   if (s1 == s0) return false;
   if (s0 < 0 || s1 < s0 || s1 > a.rows || s1 - s0 > a.max_rows) {
     if (threadIdx.x == 0) raise(a.status, kStatusRows);
@@ -481,9 +488,9 @@ __device__ __forceinline__ bool request_at(const Attend& a, int b, Request& r) {
   }
   r.row0 = s0;
   r.count = s1 - s0;
-  r.past = a.past[b];
   r.cap = clamp_int((int64_t)a.width << a.shift);
   const int64_t len = (int64_t)r.past + r.count;
+  r.past = min(r.past, INT32_MAX - r.count);  // (past any table either way; positions stay ints)
   r.len = len < 0 ? 0 : len > r.cap ? r.cap : (int)len;
   r.narrow = (int64_t)r.count * a.group <= 16;
   if (len > r.cap && threadIdx.x == 0) raise(a.status, kStatusPage);
@@ -521,7 +528,6 @@ __device__ __forceinline__ float across_sum32(float v) {
 }
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
   bf16x2 r;
   r[0] = (__bf16)a;
   r[1] = (__bf16)b;
@@ -536,12 +542,67 @@ __device__ __forceinline__ bf16x8 codes8(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(bf16x8, r);
 }
 
+// max(a, b) as the median with infinity, one instruction: fmaxf() quiets each
+// operand first, since the matrix cores' results may be anything (and does so
+// here too, if the compiler sees that it is infinity). A NaN is left out
+// beside a number; two give infinity, whose column is NaN as well.
+__device__ __forceinline__ float hidden_infinity() {
+  float x = INFINITY;
+  asm("" : "+v"(x));
+  return x;
+}
+__device__ __forceinline__ float max_of(float a, float b, float infinity) { return __builtin_amdgcn_fmed3f(a, b, infinity); }
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float nan_of() { return __uint_as_float(0x7fc00000u); }
 
-// The weight of a part whose maximum is m in a sum whose maximum is all: 0
-// for a part that saw nothing (m = -inf).
-__device__ __forceinline__ float part_weight(float m, float all) {
-  return m == -INFINITY ? 0.0f : exp2_of(m - all);
+// log2 of a value scale, whole for a power of two; -inf for one without
+// effect (0, a subnormal), NaN for one that is not finite or is negative.
+__device__ __forceinline__ float scale_log2(float s) {
+  const uint32_t u = __float_as_uint(s);
+  if ((u & 0x7f800000u) == 0u) return -INFINITY;
+  if (u >= 0x7f800000u) return nan_of();
+  const uint32_t m = u & 0x7fffffu;
+  return (float)((int)(u >> 23) - 127) + (m ? __builtin_amdgcn_logf(__uint_as_float(0x3f800000u | m)) : 0.0f);
+}
+
+// A segment's scales as the kernels use them. A page that cannot be read, or
+// a value scale that is not a number, has to be NaN to the rows that attend
+// to it and nothing to the others: the key scale carries it, since masked
+// scores are replaced, and its values count as 0.
+struct Scales {
+  float ks;  // key scale * log2(e) * softmax scale
+  float lv;  // log2 of the value scale; -inf: the values count as 0
+};
+__device__ __forceinline__ Scales scales_of(const Attend& a, size_t head, bool bad) {
+  Scales s{a.ks[head] * a.scale, scale_log2(a.vs[head])};
+  if (bad || s.lv != s.lv) s = Scales{nan_of(), -INFINITY};
+  return s;
+}
+
+// The logarithm of a segment's value scale against the largest so far (0 for
+// one whose values count as 0), and the pair of factors that takes it out of
+// the sum again. Not below 2^-64: values that small beside the largest are
+// far below its rounding, and the factors stay numbers.
+__device__ __forceinline__ float relative(float lv, float top) { return lv == -INFINITY ? 0.0f : fmaxf(lv - top, -64.0f); }
+__device__ __forceinline__ uint32_t undo(float d) {
+  const float w = exp2_of(-d);
+  return pack_bf16(w, w);
+}
+__device__ __forceinline__ float dot2(uint32_t p, uint32_t w, float sum) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p), __builtin_bit_cast(bf16x2, w), sum, false);
+}
+
+// The running statistics of a column (a query): the maximum m that its
+// exponents are against, the sum, and the largest value scale `top` (of the
+// whole wave). They move only when a score passes m by more than 2^8, or the
+// scales grow: an m below the maximum leaves every p below 2^8 and their
+// ratios as they are.
+constexpr float kSlack = 8.0f;
+
+// A part's share of a whole: its sum against the common maximum, 0 for a part
+// that saw nothing (m = -inf).
+__device__ __forceinline__ float part_weight(float m, float all, float sum) {
+  return (m == -INFINITY ? 0.0f : exp2_of(m - all)) * sum;
 }
 
 // ---- few columns: single tokens
@@ -556,7 +617,7 @@ template <int D>
 struct NarrowUnit {
   uint4 k[4][D / 64];
   uint4 v[D / 16];
-  float ks, vs;  // of this lane's segment, l / 16
+  Scales s;  // of this lane's segment, l / 16
   bool bad;
 };
 
@@ -575,20 +636,18 @@ __device__ __forceinline__ void narrow_load(const Attend& a, const int* row, int
   const uint8_t* v = a.v + ((head * D + r) << a.shift) + (at_v & (page - 1));
 #pragma unroll
   for (int t = 0; t < D / 16; ++t) x.v[t] = *reinterpret_cast<const uint4*>(v + ((size_t)(16 * t) << a.shift));
-  x.ks = a.ks[head];
-  x.vs = a.vs[head];
+  x.s = Scales{a.ks[head], a.vs[head]};  // (as they are: turned into what they are used as when they are)
 }
 
-template <int D>
+template <int D, int kWaves>
 struct NarrowShared {
-  float m[kNarrowWaves][16], l[kNarrowWaves][16];
-  float o[kNarrowWaves][16][D + 4];
+  float m[kWaves][16], l[kWaves][16];
+  float o[kWaves][16][D + 4];
 };
 
-template <int D, bool kFp8>
-__global__ void __launch_bounds__(kNarrowWaves* kWave) k_kv8_attend_narrow(const Attend a) {
-  __shared__ NarrowShared<D> sh;
-  const int h = blockIdx.x % a.kv, sp = blockIdx.x / a.kv % a.narrow_splits, b = blockIdx.x / a.kv / a.narrow_splits;
+template <int D, bool kFp8, int kWaves>
+__device__ __forceinline__ void narrow_block(const Attend& a, int index, NarrowShared<D, kWaves>& sh) {
+  const int h = index % a.kv, sp = index / a.kv % a.narrow_splits, b = index / a.kv / a.narrow_splits;
   Request rq;
   if (!request_at(a, b, rq) || !rq.narrow) return;
   const int units = (rq.len + kUnit - 1) / kUnit, per = (units + a.narrow_splits - 1) / a.narrow_splits;
@@ -601,6 +660,9 @@ __global__ void __launch_bounds__(kNarrowWaves* kWave) k_kv8_attend_narrow(const
   const int ci = r / a.group, cj = r - ci * a.group;
   const bool live = r < columns;
   const int pos = live ? rq.past + ci : -1;
+  NarrowUnit<D> next;
+  int u = u0 + w;
+  if (u < u1) narrow_load<D>(a, row, h, rq.len, u, next);
   bf16x8 q[D / 32];
   {
     const uint16_t* src = a.q + (size_t)(rq.row0 + (live ? ci : 0)) * a.q_stride + (size_t)(h * a.group + (live ? cj : 0)) * D + g * (D / 4);
@@ -612,16 +674,13 @@ __global__ void __launch_bounds__(kNarrowWaves* kWave) k_kv8_attend_narrow(const
       q[c] = __builtin_bit_cast(bf16x8, x);
     }
   }
-  float m = -INFINITY, sum = 0.0f;
+  float m = -INFINITY, sum = 0.0f, top = -INFINITY;
   f32x4 o[D / 16];
 #pragma unroll
   for (int t = 0; t < D / 16; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  NarrowUnit<D> next;
-  int u = u0 + w;
-  if (u < u1) narrow_load<D>(a, row, h, rq.len, u, next);
-  for (; u < u1; u += kNarrowWaves) {
+  for (; u < u1; u += kWaves) {
     NarrowUnit<D> x = next;
-    if (u + kNarrowWaves < u1) narrow_load<D>(a, row, h, rq.len, u + kNarrowWaves, next);
+    if (u + kWaves < u1) narrow_load<D>(a, row, h, rq.len, u + kWaves, next);
     f32x4 s[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -633,15 +692,16 @@ __global__ void __launch_bounds__(kNarrowWaves* kWave) k_kv8_attend_narrow(const
       }
     }
     const int at = u * kUnit + 16 * g;  // this lane's first position
-    const bool whole = u * kUnit + kUnit - 1 <= rq.past && __ballot(x.bad) == 0;  // seen by every column
-    if (x.bad) {
-      raise(a.status, kStatusPage);
-      x.ks = __uint_as_float(0x7fc00000u);
-    }
-    const float ks = x.ks * a.scale;
+    const bool inside = at < rq.len;
+    Scales sc{x.s.ks * a.scale, scale_log2(x.s.lv)};
+    if (x.bad) raise(a.status, kStatusPage);
+    const bool none = x.bad || !(sc.lv > -INFINITY);  // the segment's values count as 0
+    if (x.bad || sc.lv != sc.lv) sc.ks = nan_of();
+    if (none || !inside) sc.lv = -INFINITY;
+    const bool whole = u * kUnit + kUnit - 1 <= rq.past && __ballot(none) == 0;  // seen by every column
     if (!whole) {
       // values behind the last position may be anything
-      const int left = x.bad ? 0 : rq.len - at;
+      const int left = none ? 0 : rq.len - at;
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) {
         uint32_t* const v = reinterpret_cast<uint32_t*>(&x.v[t]);
@@ -661,15 +721,21 @@ __global__ void __launch_bounds__(kNarrowWaves* kWave) k_kv8_attend_narrow(const
 #pragma unroll
     for (int t = 0; t < 4; ++t) most = fmaxf(most, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
     // (a segment that the column sees nothing of has -inf here, whatever its scale)
-    most = across_max16(most == -INFINITY ? most : most * ks);
-    const float m_new = fmaxf(m, most), m_use = m_new == -INFINITY ? 0.0f : m_new;
-    if (__ballot(m_new != m) != 0) {
-      const float shrink = exp2_of(m - m_use);
+    most = across_max16(most == -INFINITY ? most : most * sc.ks);
+    const float new_top = fmaxf(top, across_max16(sc.lv));
+    if (__ballot(most > m + kSlack || new_top > top) != 0) {
+      const float m_new = fmaxf(m, most), to = m_new == -INFINITY ? 0.0f : m_new;
+      const float shrink = exp2_of(m - to), shrink_top = exp2_of(top == -INFINITY ? 0.0f : top - new_top);
       sum *= shrink;
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t) o[t] *= shrink;
+      for (int t = 0; t < D / 16; ++t) o[t] *= shrink * shrink_top;
       m = m_new;
+      top = new_top;
     }
+    const float d = relative(sc.lv, top), add = d - (m == -INFINITY ? 0.0f : m);
+    const uint32_t back = undo(d);
+    // The probabilities are rounded to BF16, the value product's operand
+    // type: up to 2^-8 of each, the same rounded ones in the sum.
     bf16x8 p[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -679,20 +745,13 @@ __global__ void __launch_bounds__(kNarrowWaves* kWave) k_kv8_attend_narrow(const
         float e[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          e[i] = exp2_of(fmaf(s[2 * c + t][i], ks, -m_use));
+          e[i] = exp2_of(fmaf(s[2 * c + t][i], sc.ks, add));
           if (!whole && at + 4 * (2 * c + t) + i > pos) e[i] = 0.0f;
-          sum += e[i];
         }
-        // the probabilities' rounding to BF16, the value product's operand
-        // type: 2^-9 of each, independent of one another
-        float f[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          f[i] = e[i] * x.vs;
-          if (!whole && at + 4 * (2 * c + t) + i > pos) f[i] = 0.0f;  // (a scale may be NaN)
-        }
-        pk[2 * t] = pack_bf16(f[0], f[1]);
-        pk[2 * t + 1] = pack_bf16(f[2], f[3]);
+        pk[2 * t] = pack_bf16(e[0], e[1]);
+        pk[2 * t + 1] = pack_bf16(e[2], e[3]);
+        sum = dot2(pk[2 * t], back, sum);
+        sum = dot2(pk[2 * t + 1], back, sum);
       }
       p[c] = __builtin_bit_cast(bf16x8, uint4{pk[0], pk[1], pk[2], pk[3]});
     }
@@ -702,60 +761,89 @@ __global__ void __launch_bounds__(kNarrowWaves* kWave) k_kv8_attend_narrow(const
       o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes8<kFp8>(x.v[t].z, x.v[t].w), p[1], o[t], 0, 0, 0);
     }
   }
-  // join the waves: o of this lane is column r, dimensions 16 t + 4 g + i
+  // Join the waves, each as its own result (so that nothing passes the range
+  // of the values): o of this lane is column r, dimensions 16 t + 4 g + i.
   sum = across_sum16(sum);
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, unit = exp2_of(top);
   if (g == 0) {
     sh.m[w][r] = m;
     sh.l[w][r] = sum;
   }
 #pragma unroll
   for (int t = 0; t < D / 16; ++t)
-    *reinterpret_cast<f32x4*>(&sh.o[w][r][16 * t + 4 * g]) = o[t];
+    *reinterpret_cast<f32x4*>(&sh.o[w][r][16 * t + 4 * g]) = o[t] * inv * unit;
   __syncthreads();
   const int heads = a.kv * a.group;
-  for (int e = threadIdx.x; e < columns * (D / 4); e += kNarrowWaves * kWave) {
+  for (int e = threadIdx.x; e < columns * (D / 4); e += kWaves * kWave) {
     const int c = e / (D / 4), d = 4 * (e % (D / 4));
     float all = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kNarrowWaves; ++i) all = fmaxf(all, sh.m[i][c]);
-    float total = 0.0f;
+    for (int i = 0; i < kWaves; ++i) all = fmaxf(all, sh.m[i][c]);
+    float share[kWaves], total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) total += share[i] = part_weight(sh.m[i][c], all, sh.l[i][c]);
     f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < kNarrowWaves; ++i) {
-      const float x = part_weight(sh.m[i][c], all);
-      total += x * sh.l[i][c];
-      acc += x * *reinterpret_cast<const f32x4*>(&sh.o[i][c][d]);
-    }
+    for (int i = 0; i < kWaves; ++i) acc += (share[i] / total) * *reinterpret_cast<const f32x4*>(&sh.o[i][c][d]);
     const int i = c / a.group, j = c - i * a.group;
     const size_t at = (size_t)(rq.row0 + i) * heads + h * a.group + j;
     if (a.narrow_splits == 1) {
-      const bool sees = rq.past + i >= 0;
       uint2 y{0, 0};
-      if (sees) y = uint2{pack_bf16(acc[0] / total, acc[1] / total), pack_bf16(acc[2] / total, acc[3] / total)};
+      if (rq.past + i >= 0) y = uint2{pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3])};
       *reinterpret_cast<uint2*>(a.out + at * D + d) = y;
     } else {
       const size_t part = (size_t)sp * a.rows * heads + at;
+      if (total == 0.0f) acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       *reinterpret_cast<f32x4*>(a.part + part * D + d) = acc;
       if (d == 0) a.part_ml[part] = float2{all, total};
     }
   }
 }
 
+template <int D, bool kFp8>
+__global__ void __launch_bounds__(kNarrowWaves* kWave, D == 64 ? 4 : 2) k_kv8_attend_narrow(const Attend a) {
+  __shared__ NarrowShared<D, kNarrowWaves> sh;
+  narrow_block<D, kFp8, kNarrowWaves>(a, blockIdx.x, sh);
+}
+
 // ---- many columns: prompt chunks
 //
 // Tiles of 128 columns of one request and KV head, a wave for 32 of them
 // (v_mfma_f32_32x32x16_bf16); a unit's keys and values are converted to BF16
-// once for all four waves, in two LDS stages, the next unit's bytes loaded
-// while this one is computed.
-constexpr int kWideWaves = 4, kWideColumns = 32 * kWideWaves, kWideThreads = kWideWaves * kWave;
+// once for four waves. Groups of four waves share a tile, each with stages of
+// its own and every third (dim 64) or second (128) unit.
+//
+// What bounds it is the vector work around the products (about 290
+// instructions a unit and wave, 80,000 of 160,000 cycles at 3,900 rows x 16
+// heads of 64) and, in what is left, the latency of one wave's chain: one
+// tile's longest chain of units decides how long a chip that holds about two
+// tiles a CU takes. Hence the groups (one group: 77 us, two: 67, three: 67,
+// and 40 -> 38 us for single tokens beside a chunk of 512), the halves of a
+// round (below), and per-segment work moved out of the unit: pages and scales
+// of 64 rounds looked up at once, a lane for each (107 -> 84 us together with
+// 32-bit offsets), nothing per score but the multiply-add, the exponential, a
+// maximum and half a conversion and half a dot product.
+constexpr int kWideWaves = 4, kWideColumns = 32 * kWideWaves;
+template <int D>
+struct Wide {
+  static constexpr int kGroups = D == 64 ? 3 : 2, kWaves = kGroups * kWideWaves, kThreads = kWaves * kWave;
+};
 
 template <int D>
-struct WideShared {
+struct WideStages {
   uint4 k[2][kUnit * (D / 8)];  // [position][dim], rows of D / 8 16-byte slots
-  uint4 v[2][D * (kUnit / 8)];  // [dim][position], scaled
-  float ks[2][4];               // the segments' key scales
+  uint4 v[D * (kUnit / 8)];     // [dim][position]
+  Scales s[4];                  // the segments'
+};
+template <int D>
+struct WideShared {
+  union {
+    WideStages<D> group[Wide<D>::kGroups];
+    f32x4 o[Wide<D>::kGroups - 1][kWideColumns][D / 4 + 1];  // the groups' results, to be joined
+  };
+  float2 ml[Wide<D>::kGroups - 1][kWideColumns];
   int found[2];
-  int waves[kWideWaves];
+  int waves[Wide<D>::kWaves];
 };
 
 // 16 rows read at one slot number spread over all 64 banks (two 128-byte rows
@@ -765,260 +853,409 @@ __device__ __forceinline__ int slot_of(int row, int c) {
   return row * kSlots + (c ^ (kSlots == 8 ? (row >> 1) & 7 : row & 15));
 }
 
+// A wave's share of a unit's staging: segment w, so that its page and scales
+// are the wave's and not each lane's. Keys: position 16 w + l / 4, 16
+// dimensions at 16 (l % 4) (and 64 more); values: dimension l (and 64 + l),
+// the segment's 16 positions. Keys run a unit ahead of values.
+//
+// The pages and scales of the wave's segments in the next 64 rounds, a lane
+// for each, looked up and made ready together.
+struct WideTable {
+  int id;     // page that may be read
+  Scales s;
+};
+
+__device__ __forceinline__ WideTable wide_table(const Attend& a, const int* row, int h, int64_t at, int end) {
+  const bool inside = at < end;
+  const int entry = inside ? row[at >> a.shift] : 0;
+  const bool bad = (uint32_t)entry >= (uint32_t)a.pages;
+  if (bad && inside) raise(a.status, kStatusPage);
+  WideTable x;
+  x.id = bad ? 0 : entry;
+  const size_t head = (size_t)x.id * a.kv + h;
+  x.s = Scales{a.ks[head] * a.scale, scale_log2(a.vs[head])};
+  if (!inside) x.s = Scales{0.0f, -INFINITY};
+  else if (bad || x.s.lv != x.s.lv) x.s = Scales{nan_of(), -INFINITY};
+  return x;
+}
+
+__device__ __forceinline__ int uniform_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ float uniform_of(float v, int lane) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
+}
+
+// A segment of this wave: where its page's head begins in either cache, its
+// scales, its first position.
+struct Segment {
+  size_t region;
+  Scales s;
+  int at;
+};
+
 template <int D>
 struct WideUnit {
   uint4 k[D / 64], v[D / 64];
-  float ks, vs[D / 64];
-  uint32_t keep;  // positions of the segment to keep in v
+  Segment of_k, of_v;
 };
 
-// This thread's share: key position t / 4, 16 dimensions at 16 (t % 4) (and
-// 64 more); value dimension t / 4 (and + 64), segment t % 4.
-template <int D>
-__device__ __forceinline__ void wide_load(const Attend& a, const int* row, int h, int end, int u, WideUnit<D>& x) {
-  const int t = threadIdx.x, page = 1 << a.shift;
-  bool bad;
-  const int at_k = u * kUnit + t / 4;
-  const int id_k = page_at(a, row, at_k, end, bad);
-  const uint8_t* k = a.k + ((((size_t)id_k * a.kv + h) << a.shift) + (at_k & (page - 1))) * D + 16 * (t & 3);
+template <int D, bool kFp8>
+__device__ __forceinline__ void store_keys(WideStages<D>& sh, int w, int stage, const WideUnit<D>& x) {
+  const int l = lane_id();
 #pragma unroll
-  for (int c = 0; c < D / 64; ++c) x.k[c] = *reinterpret_cast<const uint4*>(k + 64 * c);
-  const int at_v = u * kUnit + 16 * (t & 3);
-  const int id_v = page_at(a, row, at_v, end, bad);
-  const size_t head = (size_t)id_v * a.kv + h;
-  const uint8_t* v = a.v + ((head * D + t / 4) << a.shift) + (at_v & (page - 1));
-#pragma unroll
-  for (int c = 0; c < D / 64; ++c) x.v[c] = *reinterpret_cast<const uint4*>(v + ((size_t)(64 * c) << a.shift));
-  x.ks = a.ks[head];
-  float vs = a.vs[head];
-  const int left = end - at_v;
-  x.keep = left >= 16 ? 0xffffu : left <= 0 ? 0u : (1u << left) - 1u;
-  // A page that cannot be read, or a value scale that is not finite, is NaN to
-  // the rows that attend to it and nothing to the others: the key scale
-  // carries it, since masked scores are replaced and masked values are not.
-  if (left <= 0) x.ks = vs = 0.0f;
-  else if (bad || !(fabsf(vs) < INFINITY)) x.ks = __uint_as_float(0x7fc00000u), vs = 0.0f, x.keep = 0u;
-  if (bad) raise(a.status, kStatusPage);
-#pragma unroll
-  for (int c = 0; c < D / 64; ++c) x.vs[c] = vs;
-}
-
-template <bool kFp8>
-__device__ __forceinline__ void scaled8(uint32_t a, uint32_t b, float scale, uint4& r) {
-  float f[4];
-  Code<kFp8>::values(a, f);
-  r.x = pack_bf16(f[0] * scale, f[1] * scale);
-  r.y = pack_bf16(f[2] * scale, f[3] * scale);
-  Code<kFp8>::values(b, f);
-  r.z = pack_bf16(f[0] * scale, f[1] * scale);
-  r.w = pack_bf16(f[2] * scale, f[3] * scale);
+  for (int c = 0; c < D / 64; ++c) {
+    const int row = 16 * w + (l >> 2), at = 8 * c + 2 * (l & 3);
+    // at is even, so the two slots differ in their last bit
+    const int s = slot_of<D / 8>(row, at);
+    sh.k[stage][s] = __builtin_bit_cast(uint4, codes8<kFp8>(x.k[c].x, x.k[c].y));
+    sh.k[stage][s ^ 1] = __builtin_bit_cast(uint4, codes8<kFp8>(x.k[c].z, x.k[c].w));
+  }
 }
 
 template <int D, bool kFp8>
-__device__ __forceinline__ void wide_store(WideShared<D>& sh, int stage, WideUnit<D>& x) {
-  const int t = threadIdx.x;
+__device__ __forceinline__ void store_values(WideStages<D>& sh, int w, int end, WideUnit<D>& x) {
+  const int l = lane_id();
+  sh.s[w] = x.of_v.s;  // (every lane the same)
+  const int left = end - x.of_v.at;
+  if (left < 16 || x.of_v.s.lv == -INFINITY) {
+    // What lies behind the last position may be anything, and the values of
+    // a page or scale that is no number count as 0.
+    const int keep = x.of_v.s.lv == -INFINITY ? 0 : left;
 #pragma unroll
-  for (int c = 0; c < D / 64; ++c) {
-    const int s = 8 * c + 2 * (t & 3);
-    uint4 lo, hi;
-    lo = __builtin_bit_cast(uint4, codes8<kFp8>(x.k[c].x, x.k[c].y));
-    hi = __builtin_bit_cast(uint4, codes8<kFp8>(x.k[c].z, x.k[c].w));
-    sh.k[stage][slot_of<D / 8>(t / 4, s)] = lo;
-    sh.k[stage][slot_of<D / 8>(t / 4, s + 1)] = hi;
-    if (x.keep != 0xffffu) {
+    for (int c = 0; c < D / 64; ++c) {
       uint32_t* const v = reinterpret_cast<uint32_t*>(&x.v[c]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t n = (x.keep >> (4 * i)) & 15u;  // 0, 1, 3, 7 or 15
-        v[i] &= n == 15u ? 0xffffffffu : n == 7u ? 0xffffffu : n == 3u ? 0xffffu : n == 1u ? 0xffu : 0u;
+        const int n = keep - 4 * i;
+        v[i] &= n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
       }
     }
-    scaled8<kFp8>(x.v[c].x, x.v[c].y, x.vs[c], lo);
-    scaled8<kFp8>(x.v[c].z, x.v[c].w, x.vs[c], hi);
-    sh.v[stage][slot_of<8>(t / 4 + 64 * c, 2 * (t & 3))] = lo;
-    sh.v[stage][slot_of<8>(t / 4 + 64 * c, 2 * (t & 3) + 1)] = hi;
   }
-  if (t < 4) sh.ks[stage][t] = x.ks;
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) {
+    const int at = slot_of<8>(l + 64 * c, 2 * w);
+    sh.v[at] = __builtin_bit_cast(uint4, codes8<kFp8>(x.v[c].x, x.v[c].y));
+    sh.v[at ^ 1] = __builtin_bit_cast(uint4, codes8<kFp8>(x.v[c].z, x.v[c].w));
+  }
+}
+
+// A wave's columns and their running results.
+template <int D>
+struct WideState {
+  bf16x8 q[D / 16];
+  f32x16 o[D / 32];
+  float m, sum, top;
+};
+struct WideScores {
+  f32x16 t[2];  // positions 32 t ..
+};
+
+// The scores of one unit for one wave.
+template <int D>
+__device__ __forceinline__ void wide_scores(const WideStages<D>& sh, int stage, const WideState<D>& x, WideScores& s) {
+  const int l = lane_id(), half = l >> 5;
+  // operand row l % 32 of a key tile is position rho with bits 2 and 3
+  // exchanged: the results of lane half `half`, i = 0 .. 15, are then
+  // positions 16 (i / 8) + 8 half + i % 8
+  const int rho = (l & 0x13) | ((l & 4) << 1) | ((l & 8) >> 1);
+#pragma unroll
+  for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const bf16x8 k = __builtin_bit_cast(bf16x8, sh.k[stage][slot_of<D / 8>(32 * t + rho, 2 * c + half)]);
+      if (c == 0) s.t[t] = f32x16{};
+      s.t[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, x.q[c], s.t[t], 0, 0, 0);
+    }
+}
+
+// Those scores into the running results; kMasked: some column does not see
+// all of the unit.
+template <int D, bool kMasked>
+__device__ __forceinline__ void wide_unit(const WideStages<D>& sh, int first, int pos, bool one_page, WideScores& s,
+                                          WideState<D>& x) {
+  const int l = lane_id(), half = l >> 5;
+  Scales sc[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sc[i] = sh.s[i];
+  const int behind = pos - first - 8 * half;  // positions 32 t + 16 e + i past this are masked
+  if (kMasked) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (32 * t + 16 * (i / 8) + i % 8 > behind) s.t[t][i] = -INFINITY;
+  }
+  const float infinity = hidden_infinity();
+  float most = -INFINITY;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float v = s.t[t][8 * e];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) v = max_of(v, s.t[t][8 * e + i], infinity);
+      // (where the column sees nothing of the segment: -inf, whatever its scale)
+      most = fmaxf(most, kMasked && v == -INFINITY ? v : v * sc[2 * t + e].ks);
+    }
+  most = across_max32(most);
+  const float new_top = fmaxf(fmaxf(x.top, fmaxf(sc[0].lv, sc[1].lv)), fmaxf(sc[2].lv, sc[3].lv));
+  if (__ballot(most > x.m + kSlack || new_top > x.top) != 0) {
+    const float m_new = fmaxf(x.m, most), to = m_new == -INFINITY ? 0.0f : m_new;
+    const float shrink = exp2_of(x.m - to), shrink_top = exp2_of(x.top == -INFINITY ? 0.0f : x.top - new_top);
+    x.sum *= shrink;
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) x.o[t] *= shrink * shrink_top;
+    x.m = m_new;
+    x.top = new_top;
+  }
+  const float against = x.m == -INFINITY ? 0.0f : x.m;
+  float add[4];
+  uint32_t back[4];
+  {
+    const float d = relative(sc[0].lv, x.top);
+    add[0] = add[1] = add[2] = add[3] = d - against;
+    back[0] = back[1] = back[2] = back[3] = undo(d);
+  }
+  if (!one_page) {
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+      const float d = relative(sc[i].lv, x.top);
+      add[i] = d - against;
+      back[i] = undo(d);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        f[i] = exp2_of(fmaf(s.t[t][8 * e + i], sc[2 * t + e].ks, add[2 * t + e]));
+        if (kMasked && 32 * t + 16 * e + i > behind) f[i] = 0.0f;
+      }
+      // (rounded to BF16 as in the narrow form)
+      const uint4 pk{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])};
+      x.sum = dot2(pk.x, back[2 * t + e], x.sum);
+      x.sum = dot2(pk.y, back[2 * t + e], x.sum);
+      x.sum = dot2(pk.z, back[2 * t + e], x.sum);
+      x.sum = dot2(pk.w, back[2 * t + e], x.sum);
+      const bf16x8 p = __builtin_bit_cast(bf16x8, pk);
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        const bf16x8 v = __builtin_bit_cast(bf16x8, sh.v[slot_of<8>(32 * c + (l & 31), 4 * t + 2 * e + half)]);
+        x.o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, p, x.o[c], 0, 0, 0);
+      }
+    }
+}
+
+// The request and tile of this block's item, among the wide requests' tiles
+// in order. found: request (-1: none), tile within it.
+template <int D>
+__device__ __forceinline__ void wide_find(const Attend& a, int item, WideShared<D>& sh) {
+  const int each = (a.requests + Wide<D>::kThreads - 1) / Wide<D>::kThreads, b0 = threadIdx.x * each;
+  const int l = lane_id(), w = wave_id();
+  const auto tiles_of = [&](int b) {
+    if (b >= a.requests) return 0;
+    const int s0 = a.starts[b], s1 = a.starts[b + 1];
+    if (s0 < 0 || s1 <= s0 || s1 > a.rows || s1 - s0 > a.max_rows || (int64_t)(s1 - s0) * a.group <= 16) return 0;
+    return (int)(((int64_t)(s1 - s0) * a.group + kWideColumns - 1) / kWideColumns);
+  };
+  int mine = 0;
+  for (int j = 0; j < each; ++j) mine += tiles_of(b0 + j);
+  int upto = mine;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int x = __shfl_up(upto, d, kWave);
+    if (l >= d) upto += x;
+  }
+  if (l == kWave - 1) sh.waves[w] = upto;
+  if (threadIdx.x == 0) sh.found[0] = -1;
+  __syncthreads();
+  int total = 0;
+  for (int i = 0; i < Wide<D>::kWaves; ++i) {
+    if (i == w) upto += total;
+    total += sh.waves[i];
+  }
+  int first = upto - mine;
+  if (item >= first && item < upto) {
+    for (int j = 0; j < each; ++j) {
+      const int n = tiles_of(b0 + j);
+      if (item >= first && item < first + n) {
+        sh.found[0] = b0 + j;
+        sh.found[1] = n - 1 - (item - first);  // the longest first
+      }
+      first += n;
+    }
+  }
+  __syncthreads();
 }
 
 template <int D, bool kFp8>
-__global__ void __launch_bounds__(kWideThreads) k_kv8_attend_wide(const Attend a) {
-  __shared__ WideShared<D> sh;
-  const int h = blockIdx.x % a.kv, sp = blockIdx.x / a.kv % a.wide_splits, tile = blockIdx.x / a.kv / a.wide_splits;
+__device__ __forceinline__ void wide_block(const Attend& a, int index, WideShared<D>& sh) {
+  const int h = index % a.kv, sp = index / a.kv % a.wide_splits;
   const int w = wave_id(), l = lane_id();
-  // the request of this tile: the wide requests' tiles in order
-  {
-    const int each = (a.requests + kWideThreads - 1) / kWideThreads, b0 = threadIdx.x * each;
-    const auto tiles_of = [&](int b) {
-      if (b >= a.requests) return 0;
-      const int s0 = a.starts[b], s1 = a.starts[b + 1];
-      if (s0 < 0 || s1 <= s0 || s1 > a.rows || s1 - s0 > a.max_rows || (int64_t)(s1 - s0) * a.group <= 16) return 0;
-      return (int)(((int64_t)(s1 - s0) * a.group + kWideColumns - 1) / kWideColumns);
-    };
-    int mine = 0;
-    for (int j = 0; j < each; ++j) mine += tiles_of(b0 + j);
-    int upto = mine;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const int x = __shfl_up(upto, d, kWave);
-      if (l >= d) upto += x;
-    }
-    if (l == kWave - 1) sh.waves[w] = upto;
-    if (threadIdx.x == 0) sh.found[0] = -1;
-    __syncthreads();
-    for (int i = 0; i < w; ++i) upto += sh.waves[i];
-    int first = upto - mine;
-    if (tile >= first && tile < upto) {
-      for (int j = 0; j < each; ++j) {
-        const int n = tiles_of(b0 + j);
-        if (tile >= first && tile < first + n) {
-          sh.found[0] = b0 + j;
-          sh.found[1] = n - 1 - (tile - first);  // the longest first
-        }
-        first += n;
-      }
-    }
-    __syncthreads();
-  }
-  const int b = sh.found[0];
+  wide_find<D>(a, index / a.kv / a.wide_splits, sh);
+  const int b = __builtin_amdgcn_readfirstlane(sh.found[0]);
   if (b < 0) return;
   Request rq;
   if (!request_at(a, b, rq)) return;
   const int* row = a.table + (size_t)b * a.width;
-  const int columns = rq.count * a.group, c0 = sh.found[1] * kWideColumns;
+  const int columns = rq.count * a.group, c0 = __builtin_amdgcn_readfirstlane(sh.found[1]) * kWideColumns;
   const int last = (min(c0 + kWideColumns, columns) - 1) / a.group;  // the tile's last query row
   const int64_t end64 = (int64_t)rq.past + last + 1;
   const int end = end64 < 0 ? 0 : end64 > rq.cap ? rq.cap : (int)end64;
   const int units = (rq.len + kUnit - 1) / kUnit, per = (units + a.wide_splits - 1) / a.wide_splits;
   const int u0 = sp * per, u1 = min((end + kUnit - 1) / kUnit, u0 + per);
   if (sp > 0 && u0 >= u1) return;
+  constexpr int kGroups = Wide<D>::kGroups;
+  const int group = w / kWideWaves, w4 = w % kWideWaves;
+  WideStages<D>& mine = sh.group[group];
+  constexpr int kRound = kGroups * kUnit;            // positions of a round
+  const int first = (u0 + group) * kUnit + 16 * w4;  // this wave's first segment to stage
+  const uint32_t page_bytes = (uint32_t)((a.kv << a.shift) * D), head_bytes = (uint32_t)((h << a.shift) * D);
+  const uint32_t k_lane = (uint32_t)((l >> 2) * D + 16 * (l & 3)), v_lane = (uint32_t)(l << a.shift);
+  const int in_page = (1 << a.shift) - 1;
+  WideTable table = wide_table(a, row, h, (int64_t)first + kRound * l, end);
+  WideUnit<D> next;
+  // Loads are made for rounds past the last too (of page 0; never used).
+  const auto load_keys = [&](int i) {
+    if (i > 0 && i % kWave == 0) table = wide_table(a, row, h, (int64_t)first + (int64_t)kRound * (i + l), end);
+    next.of_v = next.of_k;
+    next.of_k.region = (size_t)(uint32_t)uniform_of(table.id, i % kWave) * page_bytes + head_bytes;
+    next.of_k.s = Scales{uniform_of(table.s.ks, i % kWave), uniform_of(table.s.lv, i % kWave)};
+    next.of_k.at = first + kRound * i;
+    const uint8_t* const k = a.k + (next.of_k.region + (uint32_t)(next.of_k.at & in_page) * D);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) next.k[c] = *reinterpret_cast<const uint4*>(k + (k_lane + 64 * c));
+  };
+  const auto load_values = [&] {
+    const uint8_t* const v = a.v + (next.of_v.region + (uint32_t)(next.of_v.at & in_page));
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) next.v[c] = *reinterpret_cast<const uint4*>(v + (v_lane + (uint32_t)((64 * c) << a.shift)));
+  };
+  load_keys(0);
   const int half = l >> 5;
-  const int column = c0 + 32 * w + (l & 31);
+  const int column = c0 + 32 * w4 + (l & 31);
   const bool live = column < columns;
   const int ci = live ? column / a.group : 0, cj = live ? column - ci * a.group : 0;
   const int pos = live ? rq.past + ci : -1;
-  bf16x8 q[D / 16];
+  WideState<D> x;
   {
     const uint16_t* src = a.q + (size_t)(rq.row0 + ci) * a.q_stride + (size_t)(h * a.group + cj) * D + 8 * half;
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
-      Pack8 x = load8(src + 16 * c);
+      Pack8 y = load8(src + 16 * c);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x.w[i] = !live ? 0u : pos >= rq.cap ? 0x7fc07fc0u : x.w[i];
-      q[c] = __builtin_bit_cast(bf16x8, x);
+      for (int i = 0; i < 4; ++i) y.w[i] = !live ? 0u : pos >= rq.cap ? 0x7fc07fc0u : y.w[i];
+      x.q[c] = __builtin_bit_cast(bf16x8, y);
     }
   }
-  float m = -INFINITY, sum = 0.0f;
-  f32x16 o[D / 32];
+  x.m = x.top = -INFINITY;
+  x.sum = 0.0f;
 #pragma unroll
-  for (int t = 0; t < D / 32; ++t)
+  for (int t = 0; t < D / 32; ++t) x.o[t] = f32x16{};
+  // Rounds (a unit for each group) that every column sees whole, then the
+  // others (the masks' registers are not held through the first loop).
+  const int wave_last = rq.past + min((c0 + 32 * w4 + 31) / a.group, rq.count - 1);  // the last position that the wave sees
+  const bool wave_live = c0 + 32 * w4 < columns;
+  const int seen = max(0, rq.past + c0 / a.group + 1) / kUnit;
+  const int rounds = (u1 - u0 + kGroups - 1) / kGroups, whole = max(0, (min(u1, seen) - u0) / kGroups);
+  const bool large = a.shift >= 6;
+  // A group's round is two halves: the unit's probabilities and value product
+  // (vector work), and the next unit's scores with the staging of what follows
+  // (matrix and LDS work): one group is in the first half while the other is
+  // in the second, a barrier apart. Keys are staged a round ahead of values.
+  const auto load = [&](int i) {  // keys of round i + 1, values of round i
+    load_keys(i + 1);
+    load_values();
+  };
+  const auto store = [&](int i) {
+    store_keys<D, kFp8>(mine, w4, (i + 1) & 1, next);
+    store_values<D, kFp8>(mine, w4, end, next);
+  };
+  WideScores s;
+  const auto stage = [&](int i) {
+    lds_barrier();
+    wide_scores<D>(mine, (i + 1) & 1, x, s);
+    store(i + 1);
+    load(i + 2);
+    lds_barrier();
+  };
+  store_keys<D, kFp8>(mine, w4, 0, next);
+  load(0);
+  if (group & 1) lds_barrier();
+  stage(-1);
+  int i = 0;
+  for (; i < whole; ++i) {
+    if (wave_live) wide_unit<D, false>(mine, 0, 0, large, s, x);
+    stage(i);
+  }
+  for (; i < rounds; ++i) {
+    const int at = (u0 + kGroups * i + group) * kUnit;
+    if (wave_live && at <= wave_last && at < u1 * kUnit) wide_unit<D, true>(mine, at, pos, large && at + kUnit <= end, s, x);
+    stage(i);
+  }
+  if (!(group & 1)) lds_barrier();
+  // join the groups, each as its own result
+  x.sum = across_sum32(x.sum);
+  const float inv = x.sum == 0.0f ? 0.0f : 1.0f / x.sum, unit = exp2_of(x.top);
+  const int c = 32 * w4 + (l & 31);
+  if (group) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
-  // the first position that some column of this wave does not see, and the
-  // last that one does
-  const int wave_first = rq.past + min((c0 + 32 * w) / a.group, rq.count - 1);
-  const int wave_last = rq.past + min((c0 + 32 * w + 31) / a.group, rq.count - 1);
-  const bool wave_live = c0 + 32 * w < columns;
-  // operand row l % 32 of a key tile is position rho with bits 2 and 3
-  // exchanged: the results of lane half `half`, i = 0 .. 15, are then
-  // positions 16 (i / 8) + 8 half + i % 8
-  const int rho = (l & 0x13) | ((l & 4) << 1) | ((l & 8) >> 1);
-  WideUnit<D> next;
-  if (u0 < u1) {
-    wide_load<D>(a, row, h, end, u0, next);
-    wide_store<D, kFp8>(sh, 0, next);
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        sh.o[group - 1][c][8 * t + 2 * i + half] = f32x4{x.o[t][4 * i], x.o[t][4 * i + 1], x.o[t][4 * i + 2], x.o[t][4 * i + 3]} * inv * unit;
+    if (half == 0) sh.ml[group - 1][c] = float2{x.m, x.sum};
   }
   __syncthreads();
-  for (int u = u0; u < u1; ++u) {
-    const int stage = (u - u0) & 1;
-    if (u + 1 < u1) wide_load<D>(a, row, h, end, u + 1, next);
-    if (wave_live && u * kUnit <= wave_last) {
-      f32x16 s[2];
+  if (group || !live) return;
+  float all = x.m;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+  for (int g = 1; g < kGroups; ++g) all = fmaxf(all, sh.ml[g - 1][c].x);
+  float share[kGroups], total = share[0] = part_weight(x.m, all, x.sum);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
+  for (int g = 1; g < kGroups; ++g) total += share[g] = part_weight(sh.ml[g - 1][c].x, all, sh.ml[g - 1][c].y);
+  const bool single = a.wide_splits == 1, none = !single && total == 0.0f;
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          const bf16x8 k = __builtin_bit_cast(bf16x8, sh.k[stage][slot_of<D / 8>(32 * t + rho, 2 * c + half)]);
-          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[c], s[t], 0, 0, 0);
-        }
-      }
-      float ks[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ks[i] = sh.ks[stage][i] * a.scale;
-      const int at = u * kUnit + 8 * half;
-      const bool whole = u * kUnit + kUnit - 1 <= wave_first;
-      if (!whole) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (at + 32 * t + 16 * (i / 8) + i % 8 > pos) s[t][i] = -INFINITY;
-      }
-      float most = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float x = s[t][8 * e];
-#pragma unroll
-          for (int i = 1; i < 8; ++i) x = fmaxf(x, s[t][8 * e + i]);
-          most = fmaxf(most, x == -INFINITY ? x : x * ks[2 * t + e]);
-        }
-      most = across_max32(most);
-      const float m_new = fmaxf(m, most), m_use = m_new == -INFINITY ? 0.0f : m_new;
-      if (__ballot(m_new != m) != 0) {
-        const float shrink = exp2_of(m - m_use);
-        sum *= shrink;
-#pragma unroll
-        for (int t = 0; t < D / 32; ++t) o[t] *= shrink;
-        m = m_new;
-      }
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float f[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            f[i] = exp2_of(fmaf(s[t][8 * e + i], ks[2 * t + e], -m_use));
-            if (!whole && at + 32 * t + 16 * e + i > pos) f[i] = 0.0f;
-            sum += f[i];
-          }
-          const bf16x8 p = __builtin_bit_cast(
-              bf16x8, uint4{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])});
-#pragma unroll
-          for (int d = 0; d < D / 32; ++d) {
-            const bf16x8 v = __builtin_bit_cast(bf16x8, sh.v[stage][slot_of<8>(32 * d + (l & 31), 4 * t + 2 * e + half)]);
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, p, o[d], 0, 0, 0);
-          }
-        }
-    }
-    if (u + 1 < u1) wide_store<D, kFp8>(sh, stage ^ 1, next);
-    __syncthreads();
-  }
-  if (!live) return;
-  sum = across_sum32(sum);
+  for (int g = 0; g < kGroups; ++g) share[g] = none ? 0.0f : share[g] / total;
   const int heads = a.kv * a.group;
   const size_t at = (size_t)(rq.row0 + ci) * heads + h * a.group + cj;
   const size_t part = (size_t)sp * a.rows * heads + at;
-  const float inv = 1.0f / sum;
 #pragma unroll
   for (int t = 0; t < D / 32; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int d = 32 * t + 8 * i + 4 * half;
-      const f32x4 x{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
-      if (a.wide_splits == 1) {
-        uint2 y{0, 0};
-        if (pos >= 0) y = uint2{pack_bf16(x[0] * inv, x[1] * inv), pack_bf16(x[2] * inv, x[3] * inv)};
-        *reinterpret_cast<uint2*>(a.out + at * D + d) = y;
+      f32x4 y = f32x4{x.o[t][4 * i], x.o[t][4 * i + 1], x.o[t][4 * i + 2], x.o[t][4 * i + 3]} * (share[0] * inv) * unit;
+#pragma unroll
+      for (int g = 1; g < kGroups; ++g) y += sh.o[g - 1][c][8 * t + 2 * i + half] * share[g];
+      if (single) {
+        uint2 z{0, 0};
+        if (pos >= 0) z = uint2{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
+        *reinterpret_cast<uint2*>(a.out + at * D + d) = z;
       } else {
-        *reinterpret_cast<f32x4*>(a.part + part * D + d) = x;
+        *reinterpret_cast<f32x4*>(a.part + part * D + d) = y;
       }
     }
-  if (a.wide_splits > 1 && half == 0) a.part_ml[part] = float2{m, sum};
+  if (!single && half == 0) a.part_ml[part] = float2{all, total};
+}
+
+// Wide tiles first, since they take longest, then the narrow requests. (LDS
+// as dynamic memory: a static array past half of a CU's makes the compiler
+// plan for 512 registers and move results between their two halves.)
+template <int D>
+union BothShared {
+  WideShared<D> wide;
+  NarrowShared<D, Wide<D>::kWaves> narrow;
+};
+
+template <int D, bool kFp8>
+__global__ void __launch_bounds__(Wide<D>::kThreads, Wide<D>::kWaves / 4) k_kv8_attend_both(const Attend a) {
+  extern __shared__ uint4 dynamic[];
+  BothShared<D>& sh = *reinterpret_cast<BothShared<D>*>(dynamic);
+  if ((int)blockIdx.x < a.wide_blocks) wide_block<D, kFp8>(a, blockIdx.x, sh.wide);
+  else narrow_block<D, kFp8, Wide<D>::kWaves>(a, blockIdx.x - a.wide_blocks, sh.narrow);
 }
 
 // ---- the parts of a split range of keys joined, in the parts' order: a wave
@@ -1045,6 +1282,11 @@ __global__ void __launch_bounds__(kCombineWaves* kWave) k_kv8_combine(const Atte
   const int heads = a.kv * a.group, l = lane_id();
   const int64_t item = (int64_t)blockIdx.x * kCombineWaves + wave_id();
   if (item >= (int64_t)a.rows * heads) return;
+  const int most = max(a.narrow_splits, a.wide_splits);
+  const size_t stride = (size_t)a.rows * heads;
+  // asked for before it is known how many parts there are
+  float2 ml{-INFINITY, 0.0f};
+  if (l < most) ml = a.part_ml[l * stride + item];
   const int x = (int)(item / heads);
   const int b = __builtin_amdgcn_readfirstlane(request_of_row(a.starts, a.requests, x));
   if (b >= a.requests) return;
@@ -1056,21 +1298,28 @@ __global__ void __launch_bounds__(kCombineWaves* kWave) k_kv8_combine(const Atte
   const int units = (rq.len + kUnit - 1) / kUnit, per = (units + splits - 1) / splits;
   const int seen = (int)((min(pos + 1, (int64_t)rq.len) + kUnit - 1) / kUnit);  // units that the row sees
   const int parts = pos < 0 ? 0 : (seen + per - 1) / per;                      // 1 .. splits, at most 64
-  const size_t stride = (size_t)a.rows * heads;
-  float2 ml{-INFINITY, 0.0f};
-  if (l < parts) ml = a.part_ml[l * stride + item];
+  if (l >= parts) ml = float2{-INFINITY, 0.0f};
   const float all = wave_max(ml.x);
-  const float weight = part_weight(ml.x, all);
-  const float total = wave_sum(weight * ml.y);
+  float share = part_weight(ml.x, all, ml.y);
+  share /= wave_sum(share);
   float acc[D / 64] = {};
-  for (int i = 0; i < parts; ++i) {
-    const float x_i = lane_value(weight, i);
+  const float* from = a.part + item * D + l;
+  constexpr int kAhead = 8;
+  for (int i0 = 0; i0 < parts; i0 += kAhead) {
+    float y[kAhead][D / 64];
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) acc[c] += x_i * a.part[(i * stride + item) * D + 64 * c + l];
+    for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) y[i][c] = from[min(i0 + i, parts - 1) * stride * D + 64 * c];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const float f = i0 + i < parts ? lane_value(share, min(i0 + i, kWave - 1)) : 0.0f;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) acc[c] += i0 + i < parts ? f * y[i][c] : 0.0f;
+    }
   }
 #pragma unroll
-  for (int c = 0; c < D / 64; ++c)
-    a.out[item * D + 64 * c + l] = pos < 0 ? (uint16_t)0 : f32_to_bf16(acc[c] / total);
+  for (int c = 0; c < D / 64; ++c) a.out[item * D + 64 * c + l] = pos < 0 ? (uint16_t)0 : f32_to_bf16(acc[c]);
 }
 
 // ------------------------------------------------------------------ host
@@ -1099,23 +1348,25 @@ struct Splits {
   bool has_wide;
 };
 
-// Parts: enough blocks to fill the chip (256 CUs, four narrow blocks or two
-// wide ones each) where the requests alone do not, of at least 256 (narrow:
-// a unit per wave) and 512 positions, from what the host knows: the lengths
-// are on the device, the table's width bounds them.
+// Parts of a request's keys, from what the host knows (the lengths are on the
+// device; the table's width bounds them): enough blocks to fill the chip (256
+// CUs, four narrow blocks or two wide ones each) where the requests alone do
+// not, of at least 256 positions (a unit for each of a narrow block's waves)
+// or 512. Beside wide tiles that fill the chip already the narrow requests
+// are divided only to keep one block's share to 8,192 positions.
 Splits splits_for(int32_t rows, int32_t requests, int32_t kv, int32_t group, int32_t max_rows, int32_t width, int32_t page) {
   Splits s{1, 1, 0, false};
   const int64_t positions = std::min<int64_t>((int64_t)width * page, INT32_MAX);
-  const auto parts = [&](int64_t blocks, int64_t wanted, int64_t least) {
-    const int64_t p = std::min((wanted + blocks - 1) / blocks, positions / least);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(p, kWave));
+  const auto parts = [&](int64_t wanted, int64_t blocks, int64_t least) {
+    return (int)std::max<int64_t>(1, std::min({wanted / blocks, positions / least, (int64_t)kWave}));
   };
-  s.narrow = parts((int64_t)std::min(requests, rows) * kv, 1024, 256);
+  s.narrow = parts(1024, (int64_t)std::min(requests, rows) * kv, 256);
   s.has_wide = (int64_t)max_rows * group > 16;
   if (s.has_wide) {
     const int64_t columns = (int64_t)rows * group;
     s.wide_tiles = columns / kWideColumns + std::min<int64_t>(requests, columns / 17 + 1);
-    s.wide = parts(s.wide_tiles * kv, 512, 512);
+    s.wide = parts(512, s.wide_tiles * kv, 512);
+    if (s.wide_tiles * kv >= 256) s.narrow = (int)std::min<int64_t>(s.narrow, (positions + 8191) / 8192);
   }
   return s;
 }
@@ -1127,10 +1378,12 @@ size_t part_floats(const Splits& s, int64_t rows, int64_t heads, int64_t dim) {
 
 template <int D, bool kFp8>
 int attend(const Attend& a, const Splits& s, hipStream_t stream) {
-  const int64_t narrow = (int64_t)a.requests * a.kv * a.narrow_splits, wide = s.wide_tiles * a.kv * a.wide_splits;
-  hipLaunchKernelGGL((k_kv8_attend_narrow<D, kFp8>), dim3((unsigned)narrow), dim3(kNarrowWaves * kWave), 0, stream, a);
+  const int64_t narrow = (int64_t)a.requests * a.kv * a.narrow_splits;
   if (s.has_wide)
-    hipLaunchKernelGGL((k_kv8_attend_wide<D, kFp8>), dim3((unsigned)wide), dim3(kWideThreads), 0, stream, a);
+    hipLaunchKernelGGL((k_kv8_attend_both<D, kFp8>), dim3((unsigned)(a.wide_blocks + narrow)), dim3(Wide<D>::kThreads),
+                       sizeof(BothShared<D>), stream, a);
+  else
+    hipLaunchKernelGGL((k_kv8_attend_narrow<D, kFp8>), dim3((unsigned)narrow), dim3(kNarrowWaves * kWave), 0, stream, a);
   if (a.narrow_splits > 1 || a.wide_splits > 1) {
     const int64_t items = (int64_t)a.rows * a.kv * a.group;
     hipLaunchKernelGGL((k_kv8_combine<D>), dim3((unsigned)((items + kCombineWaves - 1) / kCombineWaves)),
@@ -1246,6 +1499,7 @@ extern "C" int lfm25_kv8_attention(const uint16_t* query, int64_t query_stride, 
   a.width = width, a.rows = rows, a.kv = kv_heads, a.group = heads / kv_heads, a.pages = pages, a.shift = page_shift(page);
   a.requests = requests, a.max_rows = max_rows;
   a.narrow_splits = s.narrow, a.wide_splits = s.wide;
+  a.wide_blocks = (int)(s.wide_tiles * kv_heads * s.wide);
   a.scale = scale * 1.4426950408889634f;
   if (head_dim == 64) return format == LFM25_KV8_FP8 ? attend<64, true>(a, s, stream) : attend<64, false>(a, s, stream);
   return format == LFM25_KV8_FP8 ? attend<128, true>(a, s, stream) : attend<128, false>(a, s, stream);
