@@ -607,9 +607,19 @@ int lfm25_batch_linear(const uint16_t* x, const uint16_t* w, uint16_t* y, int32_
  * still find what they need only if they need no page. next_cursor: int64
  * [2], the cursor after the call; it may be cursor itself. A cursor whose
  * difference is not in [0, ring] is taken for an empty pool. */
-int lfm25_kv8_plan(const int32_t* past, const int32_t* counts, int32_t requests, int32_t* block_table, int32_t width,
-                   int32_t* free_pages, int32_t ring, const int64_t* cursor, int32_t* row_starts, int32_t* slots,
-                   int32_t rows, int64_t* next_cursor, int32_t* status, int32_t page, lfm25_stream_t stream);
+typedef struct lfm25_kv8_plan_call {
+  const int32_t* past;
+  const int32_t* counts;
+  int32_t* block_table;
+  int32_t* free_pages;
+  const int64_t* cursor;
+  int32_t* row_starts;
+  int32_t* slots;
+  int64_t* next_cursor;
+  int32_t* status;
+  int32_t requests, width, ring, rows, page;
+} lfm25_kv8_plan_call;
+int lfm25_kv8_plan(const lfm25_kv8_plan_call* c, lfm25_stream_t stream);
 
 /* New keys and values into the cache: row r ([kv_heads x head_dim] BF16 at
  * keys + r * key_stride, in elements, a multiple of 8; values alike) goes to
@@ -625,10 +635,18 @@ int lfm25_kv8_plan(const int32_t* past, const int32_t* counts, int32_t requests,
  * Codes are round-to-nearest-even of value / scale; magnitudes past 1.875 *
  * 2^127 count as that. A value that is not finite makes the scale NaN, until
  * the page is begun anew. */
-int lfm25_kv8_append(const uint16_t* keys, int64_t key_stride, const uint16_t* values, int64_t value_stride,
-                     const int32_t* slots, int32_t rows, void* key_cache, void* value_cache, float* key_scales,
-                     float* value_scales, int32_t pages, int32_t page, int32_t kv_heads, int32_t head_dim,
-                     int32_t format, lfm25_stream_t stream);
+typedef struct lfm25_kv8_append_call {
+  const uint16_t* keys;
+  const uint16_t* values;
+  const int32_t* slots;
+  void* key_cache;
+  void* value_cache;
+  float* key_scales;
+  float* value_scales;
+  int64_t key_stride, value_stride;
+  int32_t rows, pages, page, kv_heads, head_dim, format;
+} lfm25_kv8_append_call;
+int lfm25_kv8_append(const lfm25_kv8_append_call* c, lfm25_stream_t stream);
 
 /* Causal attention of the pass's rows over the cache: row i of request b
  * attends to positions 0 .. past[b] + i (its own included: append first) with
@@ -647,11 +665,24 @@ int lfm25_kv8_append(const uint16_t* keys, int64_t key_stride, const uint16_t* v
  * overlap. output must not overlap the inputs. */
 size_t lfm25_kv8_attention_workspace_bytes(int32_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim,
                                            int32_t requests, int32_t max_rows, int32_t width, int32_t page);
-int lfm25_kv8_attention(const uint16_t* query, int64_t query_stride, const void* key_cache, const void* value_cache,
-                        const float* key_scales, const float* value_scales, const int32_t* block_table, int32_t width,
-                        const int32_t* past, const int32_t* row_starts, int32_t requests, uint16_t* output, int32_t rows,
-                        int32_t heads, int32_t max_rows, float scale, int32_t pages, int32_t page, int32_t kv_heads,
-                        int32_t head_dim, int32_t format, int32_t* status, void* workspace, lfm25_stream_t stream);
+typedef struct lfm25_kv8_attention_call {
+  const uint16_t* query;
+  const void* key_cache;
+  const void* value_cache;
+  const float* key_scales;
+  const float* value_scales;
+  const int32_t* block_table;
+  const int32_t* past;
+  const int32_t* row_starts;
+  uint16_t* output;
+  int32_t* status;
+  void* workspace;
+  int64_t query_stride;
+  int32_t width, requests, rows, heads, max_rows, pages, page, kv_heads, head_dim, format;
+  int32_t reserved; /* 0 */
+  float scale;
+} lfm25_kv8_attention_call;
+int lfm25_kv8_attention(const lfm25_kv8_attention_call* c, lfm25_stream_t stream);
 
 /* ------------------------------------------------------------ Parakeet encoder
  *

@@ -22,7 +22,6 @@ CTL_POSITION, CTL_TOKEN, CTL_STATUS = 0, 1, 2
 
 _p = ctypes.c_void_p
 _i32 = ctypes.c_int32
-_i64 = ctypes.c_int64
 _i64p = ctypes.POINTER(ctypes.c_int64)
 _size = ctypes.c_size_t
 
@@ -129,11 +128,11 @@ SIGNATURES = {
     "lfm25_batch_decode": (ctypes.c_int, [ctypes.POINTER(Batch), _p, _p, _i32, _p, _p]),
     "lfm25_batch_decode_hidden": (ctypes.c_int, [ctypes.POINTER(Batch), _p, _p, _i32, _p, _p, _p]),
     "lfm25_batch_linear": (ctypes.c_int, [_p, _p, _p, _i32, _i32, _i32, _p]),
-    "lfm25_kv8_plan": (ctypes.c_int, [_p, _p, _i32, _p, _i32, _p, _i32, _p, _p, _p, _i32, _p, _p, _i32, _p]),
-    "lfm25_kv8_append": (ctypes.c_int, [_p, _i64, _p, _i64, _p, _i32, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _p]),
+    # (the kv8 calls' structures are packed by ops.py, as bytes)
+    "lfm25_kv8_plan": (ctypes.c_int, [ctypes.c_char_p, _p]),
+    "lfm25_kv8_append": (ctypes.c_int, [ctypes.c_char_p, _p]),
     "lfm25_kv8_attention_workspace_bytes": (_size, [_i32] * 8),
-    "lfm25_kv8_attention": (ctypes.c_int, [_p, _i64, _p, _p, _p, _p, _p, _i32, _p, _p, _i32, _p, _i32, _i32, _i32,
-                                           ctypes.c_float, _i32, _i32, _i32, _i32, _i32, _p, _p, _p]),
+    "lfm25_kv8_attention": (ctypes.c_int, [ctypes.c_char_p, _p]),
     "lfm25_pk_gemm": (ctypes.c_int, [_p, _i32, _p, _i32, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _p, _p]),
     "lfm25_pk_layer_norm": (ctypes.c_int, [_p, _p, ctypes.c_float, _p, _p, _p, _p, _i32, _p, _i32, _p]),
     "lfm25_pk_attention": (ctypes.c_int, [_p, _p, _p, _p, _i32, _i32, _i32, _p]),

@@ -25,34 +25,24 @@ constexpr int kStatusRows = 2;  // attention: row offsets outside the rows, or m
 // With P the page size: held = ceil(past / P), after = ceil((past + count) /
 // P), need = after - held; an exclusive sum of the needs indexes the free
 // ring. One block, so that the cursor may be updated in place and every
-// read of the ring comes before the cursor moves; requests four to a thread,
-// rows and pages one to a thread, each finding its request by bisection of
-// the sums in LDS.
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanEach = kMaxRequests / kPlanThreads;
+// read of the ring comes before the cursor moves; requests up to four to a
+// thread, rows and pages one to a thread, each finding its request by
+// bisection of the sums in LDS. The sums saturate at 2^31 - 1, which no
+// request that is served comes near.
+constexpr int kPlanRows = 8192;  // more rows than this get their slots from k_kv8_slots
 
-struct Sums {
-  int64_t a, b;
-};
-
-// Exclusive sums over the block's threads; *total = the whole sums.
-__device__ __forceinline__ Sums block_sums(Sums v, Sums* waves, Sums* total) {
-  Sums s = v;
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const int64_t a = __shfl_up(s.a, d, kWave), b = __shfl_up(s.b, d, kWave);
-    if (lane_id() >= d) s.a += a, s.b += b;
-  }
-  __syncthreads();  // the sums of a call before are read
-  if (lane_id() == kWave - 1) waves[wave_id()] = s;
-  __syncthreads();
-  Sums before{0, 0}, all{0, 0};
-  for (int w = 0; w < kPlanThreads / kWave; ++w) {
-    if (w == wave_id()) before = all;
-    all.a += waves[w].a, all.b += waves[w].b;
-  }
-  *total = all;
-  return Sums{before.a + s.a - v.a, before.b + s.b - v.b};
+// Inclusive sums over the wave's lanes.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int dpp_add_sat(int v) {
+  return __builtin_elementwise_add_sat(v, __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xf, false));
+}
+__device__ __forceinline__ int wave_sums(int v) {
+  v = dpp_add_sat<0x111, 0xf>(v);  // within a row of 16 lanes: from 1, 2, 4, 8 lanes below
+  v = dpp_add_sat<0x112, 0xf>(v);
+  v = dpp_add_sat<0x114, 0xf>(v);
+  v = dpp_add_sat<0x118, 0xf>(v);
+  v = dpp_add_sat<0x142, 0xa>(v);  // the last lane of rows 0 and 2 to rows 1 and 3
+  return dpp_add_sat<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
 }
 
 // The last index i of at[0 .. n] with at[i] <= x (at[0] = 0 <= x).
@@ -66,51 +56,77 @@ __device__ __forceinline__ int last_not_above(const int* at, int n, int x) {
   return lo;
 }
 
+template <int kMost>
 struct PlanShared {
-  Sums waves[kPlanThreads / kWave];
-  int starts[kMaxRequests + 1];  // first row of each request
-  int takes[kMaxRequests + 1];   // pages taken before each request
-  int gives[kMaxRequests + 1];   // pages given back before each request
-  uint8_t status[kMaxRequests];
+  int waves[2][16];
+  int taken, given;
+  int starts[kMost + 1];  // first row of each request
+  int takes[kMost + 1];   // pages taken before each request
+  int gives[kMost + 1];   // pages given back before each request
+  int past[kMost];
+  uint8_t status[kMost];
 };
 
 __device__ __forceinline__ int clamp_int(int64_t v) { return v > INT32_MAX ? INT32_MAX : (int)v; }
 
-__global__ void __launch_bounds__(kPlanThreads) k_kv8_plan(const int* __restrict__ past, const int* __restrict__ counts,
-                                                           int n, int* table, int width, int* ring, int ring_n,
-                                                           const int64_t* cursor, int* __restrict__ row_starts,
-                                                           int* __restrict__ slots, int rows, int64_t* next_cursor,
-                                                           int* __restrict__ status, int shift) {
-  __shared__ PlanShared sh;
+// Exclusive sum over the block's threads; *total = the whole sum.
+template <int kThreads>
+__device__ __forceinline__ int block_sums(int v, int* waves, int& total) {
+  const int upto = wave_sums(v);
+  // the lane below's, not upto - v: the sum may have saturated
+  const int below = __builtin_amdgcn_update_dpp(0, upto, 0x138, 0xf, 0xf, false);
+  if (kThreads == kWave) {
+    total = __builtin_amdgcn_readlane(upto, kWave - 1);
+    return below;
+  }
+  if (lane_id() == kWave - 1) waves[wave_id()] = upto;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / kWave; ++w) {
+    if (w == wave_id()) before = all;
+    all = __builtin_elementwise_add_sat(all, waves[w]);
+  }
+  total = all;
+  return __builtin_elementwise_add_sat(before, below);
+}
+
+// kThreads threads, requests up to kEach a thread.
+template <int kThreads, int kEach>
+__global__ void __launch_bounds__(kThreads) k_kv8_plan(const int* __restrict__ past, const int* __restrict__ counts, int n,
+                                                       int* table, int width, int* ring, int ring_n, const int64_t* cursor,
+                                                       int* __restrict__ row_starts, int* __restrict__ slots, int rows,
+                                                       int64_t* next_cursor, int* __restrict__ status, int shift) {
+  extern __shared__ uint4 dynamic[];
+  PlanShared<kThreads * kEach>& sh = *reinterpret_cast<PlanShared<kThreads * kEach>*>(dynamic);
   const int t = threadIdx.x, page = 1 << shift;
+  int p[kEach], c[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int b = t * kEach + j;
+    p[j] = b < n ? past[b] : 0;
+    c[j] = b < n ? counts[b] : 0;
+  }
   const int64_t taken = cursor[0], given = cursor[1];
   const int64_t window = given - taken;
   const bool sound_ring = taken >= 0 && window >= 0 && window <= ring_n;
-  const int64_t free = sound_ring ? window : 0;
-  const int each = (n + kPlanThreads - 1) / kPlanThreads;
-  int p[kPlanEach], c[kPlanEach];
-  Sums v{0, 0}, total;
-  for (int j = 0; j < kPlanEach; ++j) {
-    const int b = t * each + j;
-    p[j] = c[j] = 0;
-    if (j < each && b < n) {
-      p[j] = past[b];
-      c[j] = counts[b];
-      v.a += c[j] > 0 ? c[j] : 0;
-    }
-  }
-  int64_t row = block_sums(v, sh.waves, &total).a;
-  const int64_t all_rows = total.a;
+  const int free = sound_ring ? (int)window : 0;
+  int v = 0, all_rows, total;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) v = __builtin_elementwise_add_sat(v, max(c[j], 0));
+  if (t == 0) sh.taken = sh.given = 0;
+  int row = block_sums<kThreads>(v, sh.waves[0], all_rows);
   // what each request asks for; the row offsets decide which fit the rows
-  int need[kPlanEach], give[kPlanEach], why[kPlanEach];
-  v = Sums{0, 0};
-  for (int j = 0; j < kPlanEach; ++j) {
-    const int b = t * each + j;
+  int need[kEach], give[kEach], why[kEach], needs = 0, gifts = 0;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int b = t * kEach + j;
     need[j] = give[j] = why[j] = 0;
-    if (j >= each || b >= n) continue;
-    sh.starts[b] = clamp_int(row);
+    if (b >= n) continue;
+    sh.starts[b] = row;
+    sh.past[b] = p[j];
+    row = __builtin_elementwise_add_sat(row, max(c[j], 0));
     const int64_t held = ((int64_t)p[j] + page - 1) >> shift;
-    row += c[j] > 0 ? c[j] : 0;
     if (p[j] < 0 || held > width) {
       why[j] = LFM25_KV8_LENGTH;
     } else if (c[j] < 0) {
@@ -121,66 +137,113 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv8_plan(const int* __restrict
       else if (c[j] > 0 && row > rows) why[j] = LFM25_KV8_ROWS;
       else need[j] = (int)(after - held);
     }
-    v.a += need[j], v.b += give[j];
+    needs = __builtin_elementwise_add_sat(needs, need[j]);
+    gifts = __builtin_elementwise_add_sat(gifts, give[j]);
   }
-  const Sums before = block_sums(v, sh.waves, &total);
-  int64_t take = before.a, back = before.b;
+  int take = block_sums<kThreads>(needs, sh.waves[1], total);
+  if (t == 0) sh.takes[n] = total, sh.starts[n] = all_rows, row_starts[n] = all_rows;
+  int back = block_sums<kThreads>(gifts, sh.waves[0], total);  // (everyone has read its sums of rows)
+  if (t == 0) sh.gives[n] = total;
   // The sums only grow, so every request after the first that the pool cannot
-  // serve is refused too, if it needs a page: the first `mine` pages go to
-  // the requests served, in order.
-  v = Sums{0, 0};
-  for (int j = 0; j < kPlanEach; ++j) {
-    const int b = t * each + j;
-    if (j >= each || b >= n) continue;
-    sh.takes[b] = clamp_int(take);
-    sh.gives[b] = clamp_int(back);
-    take += need[j], back += give[j];
-    if (need[j] > 0 && take > free) why[j] = LFM25_KV8_POOL;
-    if (give[j] > 0 && (!sound_ring || free + back > ring_n)) why[j] = LFM25_KV8_POOL;
-    if (!why[j]) v.a += need[j], v.b += give[j];
+  // serve is refused too, if it needs a page: the pages up to the last one
+  // served go to the requests served, in order.
+  int last_take = 0, last_back = 0;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int b = t * kEach + j;
+    if (b >= n) continue;
+    sh.takes[b] = take;
+    sh.gives[b] = back;
+    take = __builtin_elementwise_add_sat(take, need[j]);
+    back = __builtin_elementwise_add_sat(back, give[j]);
+    if (need[j] > 0) {
+      if (take > free) why[j] = LFM25_KV8_POOL;
+      else last_take = take;
+    }
+    if (give[j] > 0) {
+      if (!sound_ring || (int64_t)free + back > ring_n) why[j] = LFM25_KV8_POOL;
+      else last_back = back;
+    }
     sh.status[b] = (uint8_t)why[j];
     status[b] = why[j];
     row_starts[b] = sh.starts[b];
   }
-  if (t == 0) {
-    sh.starts[n] = clamp_int(all_rows);
-    sh.takes[n] = clamp_int(total.a);
-    sh.gives[n] = clamp_int(total.b);
-    row_starts[n] = clamp_int(all_rows);
-  }
-  block_sums(v, sh.waves, &total);  // (its barriers also publish the sums above)
-  const int mine = (int)total.a, returned = (int)total.b;
-  const int head = sound_ring ? (int)(taken % ring_n) : 0, tail = sound_ring ? (int)(given % ring_n) : 0;
+  if (last_take > 0) atomicMax(&sh.taken, last_take);
+  if (last_back > 0) atomicMax(&sh.given, last_back);
+  __syncthreads();
+  const int mine = sh.taken, returned = sh.given;
+  const auto place = [&](int64_t at) {  // ring entry of a counter
+    return at <= INT32_MAX ? (int)((uint32_t)at % (uint32_t)ring_n) : (int)(at % ring_n);
+  };
+  const int head = sound_ring ? place(taken) : 0, tail = sound_ring ? place(given) : 0;
   const auto at = [&](int from, int k) {  // ring entry k past `from`, k <= ring_n
     const int64_t i = (int64_t)from + k;
     return (int)(i >= ring_n ? i - ring_n : i);
   };
-  for (int k = t; k < mine; k += kPlanThreads) {
+  const auto held_by = [&](int b) { return (int)(((int64_t)sh.past[b] + page - 1) >> shift); };
+  for (int k = t; k < mine; k += kThreads) {
     const int b = last_not_above(sh.takes, n, k);
-    const int held = (int)(((int64_t)past[b] + page - 1) >> shift);
-    table[(size_t)b * width + held + (k - sh.takes[b])] = ring[at(head, k)];
+    table[(size_t)b * width + held_by(b) + (k - sh.takes[b])] = ring[at(head, k)];
   }
-  for (int k = t; k < returned; k += kPlanThreads) {
+  for (int k = t; k < returned; k += kThreads) {
     const int b = last_not_above(sh.gives, n, k);
     ring[at(tail, k)] = table[(size_t)b * width + (k - sh.gives[b])];
   }
-  for (int r = t; r < rows; r += kPlanThreads) {
-    int slot = -1;
-    if (r < all_rows) {
-      const int b = last_not_above(sh.starts, n, r);
-      if (b < n && !sh.status[b]) {
-        const int first = past[b], pos = first + (r - sh.starts[b]);
-        const int held = (int)(((int64_t)first + page - 1) >> shift), i = pos >> shift;
-        const int id = i < held ? table[(size_t)b * width + i] : ring[at(head, sh.takes[b] + i - held)];
-        if (id >= 0 && id <= (INT32_MAX >> shift)) slot = id * page + (pos & (page - 1));
+  if (rows <= kPlanRows) {
+    // Four rows at a time, their page numbers asked for together. (From the
+    // ring where they are new: another thread may not have put them into the
+    // table yet.)
+    constexpr int kAhead = 4;
+    for (int r0 = t; r0 < rows; r0 += kAhead * kThreads) {
+      int id[kAhead], in_page[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int r = r0 + i * kThreads;
+        id[i] = -1;
+        if (r < min(rows, all_rows)) {
+          const int b = last_not_above(sh.starts, n, r);
+          if (b < n && !sh.status[b]) {
+            const int pos = sh.past[b] + (r - sh.starts[b]), held = held_by(b), e = pos >> shift;
+            in_page[i] = pos & (page - 1);
+            id[i] = e < held ? table[(size_t)b * width + e] : ring[at(head, sh.takes[b] + e - held)];
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int r = r0 + i * kThreads;
+        if (r < rows) slots[r] = id[i] >= 0 && id[i] <= (INT32_MAX >> shift) ? id[i] * page + in_page[i] : -1;
       }
     }
-    slots[r] = slot;
   }
   if (t == 0) {
     next_cursor[0] = taken + mine;
     next_cursor[1] = given + returned;
   }
+}
+
+// Slots of many rows, from what k_kv8_plan wrote, a row a thread.
+constexpr int kSlotThreads = 256;
+
+__global__ void __launch_bounds__(kSlotThreads) k_kv8_slots(const int* __restrict__ past, int n, const int* __restrict__ table,
+                                                            int width, const int* __restrict__ row_starts,
+                                                            const int* __restrict__ status, int* __restrict__ slots, int rows,
+                                                            int shift) {
+  __shared__ int starts[kMaxRequests + 1];
+  for (int i = threadIdx.x; i <= n; i += kSlotThreads) starts[i] = row_starts[i];
+  __syncthreads();
+  const int r = blockIdx.x * kSlotThreads + threadIdx.x;
+  if (r >= rows) return;
+  int slot = -1;
+  const int b = last_not_above(starts, n, r);
+  if (b < n) {
+    const int refused = status[b], first = past[b];
+    if (!refused) {
+      const int pos = first + (r - starts[b]), id = table[(size_t)b * width + (pos >> shift)];
+      if (id >= 0 && id <= (INT32_MAX >> shift)) slot = (id << shift) + (pos & ((1 << shift) - 1));
+    }
+  }
+  slots[r] = slot;
 }
 
 // ------------------------------------------------------------------ 8-bit codes
@@ -267,156 +330,243 @@ __device__ __forceinline__ float scale_for(uint32_t largest) {
 }
 
 struct AppendShared {
-  uint32_t largest[kAppendThreads / kWave];
+  int largest[kAppendThreads / kWave];
 };
 
-// One run of rows [r0, r0 + len) (positions off .. off + len of one page) of
-// one KV head, keys (which = 0) or values, by `team` waves, this one number
-// `member`. Teams of more than one wave meet at block barriers.
-template <int D, bool kFp8, int kTeam>
-__device__ __forceinline__ void append_run(const Append& a, AppendShared& sh, int which, int member, int h, int id, int off,
-                                           int r0, int len) {
-  const int l = lane_id(), tid = member * kWave + l, threads = kTeam * kWave, page = 1 << a.shift;
-  const size_t region = ((size_t)id * a.kv + h) * (size_t)D << a.shift;
-  uint8_t* const cache = a.cache[which] + region;
-  float* const scale_at = a.scales[which] + (size_t)id * a.kv + h;
-  const uint16_t* const x = a.x[which] + (size_t)r0 * a.stride[which] + (size_t)h * D;
-  const int64_t stride = a.stride[which];
-  const float old = off > 0 ? *scale_at : 0.0f;
-  // the largest magnitude, on the BF16 bits: what is not finite is past 0x7f80
-  constexpr int kPer = D / 8;
-  uint32_t largest = 0;
-  for (int u = tid; u < len * kPer; u += threads) {
-    const Pack8 w = load8(x + (u / kPer) * stride + 8 * (u % kPer));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) largest = max(largest, max(w.w[i] & 0x7fffu, (w.w[i] >> 16) & 0x7fffu));
-  }
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) largest = max(largest, (uint32_t)__shfl_xor((int)largest, d, kWave));
-  if (kTeam > 1) {
-    if (l == 0) sh.largest[which * kTeam + member] = largest;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kTeam; ++i) largest = max(largest, sh.largest[which * kTeam + i]);
-    __syncthreads();  // read before the next run writes
-  }
-  const bool lost = largest >= 0x7f80u || old != old;  // not finite, or the page was lost before
-  const float scale = lost ? __uint_as_float(0x7fc00000u) : fmaxf(old, scale_for<kFp8>(largest));
-  const bool grows = !lost && off > 0 && scale > old;
-  const float ratio = grows ? old / scale : 1.0f;
-  if (tid == 0 && (off == 0 || lost || grows)) *scale_at = scale;
-  const auto code_of = [&](uint32_t bits16) {
+__device__ __forceinline__ int wave_max_int(int v) {
+  v = max(v, __builtin_amdgcn_mov_dpp(v, kDppQuadXor1, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_mov_dpp(v, kDppQuadXor2, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_mov_dpp(v, kDppRowHalfMirror, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_mov_dpp(v, kDppRowMirror, 0xf, 0xf, true));
+  return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+             max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+
+// The largest of a page's magnitude and the page's scale before and after.
+struct PageScale {
+  float scale, ratio;
+  bool lost, grows;
+  __device__ __forceinline__ float value(uint32_t bits16) const {
     const float v = fminf(fmaxf(bf16_to_f32(bits16), -kLargest), kLargest);
     return lost ? 0.0f : v / scale;
-  };
-  const auto moved = [&](uint32_t w) {
-    float f[4];
-    Code<kFp8>::values(w, f);
-    return Code<kFp8>::four(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
-  };
-  if (which == 0) {
-    for (int u = tid; u < len * kPer; u += threads) {
-      const int r = u / kPer, d = 8 * (u % kPer);
-      const Pack8 w = load8(x + r * stride + d);
-      uint2 c;
-      c.x = Code<kFp8>::four(code_of(w.w[0] & 0xffffu), code_of(w.w[0] >> 16), code_of(w.w[1] & 0xffffu), code_of(w.w[1] >> 16));
-      c.y = Code<kFp8>::four(code_of(w.w[2] & 0xffffu), code_of(w.w[2] >> 16), code_of(w.w[3] & 0xffffu), code_of(w.w[3] >> 16));
-      *reinterpret_cast<uint2*>(cache + (size_t)(off + r) * D + d) = c;
-    }
-    if (grows) {
-      for (int u = tid; u < off * (D / 16); u += threads) {
-        uint4 w = *reinterpret_cast<const uint4*>(cache + (size_t)u * 16);
-        w.x = moved(w.x), w.y = moved(w.y), w.z = moved(w.z), w.w = moved(w.w);
-        *reinterpret_cast<uint4*>(cache + (size_t)u * 16) = w;
-      }
-    }
-    return;
   }
-  // Values: a thread owns two dimensions of 16 positions (32 bytes), so no
-  // byte has two writers: whole new segments and changed old ones as 16-byte
-  // stores, a few new positions as bytes.
-  const int s0 = grows ? 0 : off >> 4, s1 = (off + len + 15) >> 4;
-  for (int u = tid; u < (s1 - s0) * (D / 2); u += threads) {
-    const int seg = s0 + u / (D / 2), d = 2 * (u % (D / 2)), p0 = 16 * seg;
-    uint32_t w[16];
+};
+
+// `largest`: this thread's largest magnitude, as BF16 bits (which order as the
+// values do; what is not finite is past 0x7f80). Teams of four waves meet here.
+template <bool kFp8, int kTeam>
+__device__ __forceinline__ PageScale page_scale(AppendShared& sh, int tid, uint32_t largest, float old, int off, float* scale_at) {
+  int most = wave_max_int((int)largest);
+  if (kTeam > 1) {
+    if (lane_id() == 0) sh.largest[tid / kWave] = most;
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int r = p0 + i - off;
-      w[i] = r >= 0 && r < len ? *reinterpret_cast<const uint32_t*>(x + r * stride + d) : 0u;
+    for (int i = 0; i < kTeam; ++i) most = max(most, sh.largest[i]);
+    __syncthreads();  // read before the next run writes
+  }
+  PageScale p;
+  p.lost = most >= 0x7f80 || old != old;  // not finite, or the page was lost before
+  p.scale = p.lost ? __uint_as_float(0x7fc00000u) : fmaxf(old, scale_for<kFp8>((uint32_t)most));
+  p.grows = !p.lost && off > 0 && p.scale > old;
+  p.ratio = p.grows ? old / p.scale : 1.0f;
+  if (tid == 0 && (off == 0 || p.lost || p.grows)) *scale_at = p.scale;
+  return p;
+}
+
+template <bool kFp8>
+__device__ __forceinline__ uint32_t moved(uint32_t w, float ratio) {
+  float f[4];
+  Code<kFp8>::values(w, f);
+  return Code<kFp8>::four(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
+}
+
+__device__ __forceinline__ uint32_t largest_of(uint32_t w, uint32_t so_far) {
+  return max(so_far, max(w & 0x7fffu, (w >> 16) & 0x7fffu));
+}
+
+// A run: rows [r0, r0 + len), at positions off .. off + len of page id.
+struct Run {
+  int r0, len, id, off;
+};
+
+// A run's keys of KV head h by kTeam waves: 8 dimensions of a row a thread
+// and unit; the first kKept units' values stay in registers between the
+// maximum and the codes, the others are read again.
+template <int D, bool kFp8, int kTeam>
+__device__ __forceinline__ void append_keys(const Append& a, AppendShared& sh, int h, const Run& run, int tid) {
+  constexpr int kPer = D / 8, kThreads = kTeam * kWave, kKept = 4;
+  uint8_t* const cache = a.cache[0] + (((size_t)run.id * a.kv + h) * (size_t)D << a.shift);
+  float* const scale_at = a.scales[0] + (size_t)run.id * a.kv + h;
+  const int64_t stride = a.stride[0];
+  const uint16_t* const x = a.x[0] + (size_t)run.r0 * stride + (size_t)h * D;
+  const int units = run.len * kPer;
+  const auto read = [&](int u) { return load8(x + (u / kPer) * stride + 8 * (u % kPer)); };
+  Pack8 kept[kKept];
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) kept[i] = read(min(tid + i * kThreads, units - 1));
+  const float old = run.off > 0 ? *scale_at : 0.0f;
+  uint32_t largest = 0;
+#pragma unroll
+  for (int i = 0; i < kKept; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) largest = largest_of(kept[i].w[k], largest);
+  for (int u = tid + kKept * kThreads; u < units; u += kThreads) {
+    const Pack8 w = read(u);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) largest = largest_of(w.w[k], largest);
+  }
+  const PageScale p = page_scale<kFp8, kTeam>(sh, tid, largest, old, run.off, scale_at);
+  const auto write = [&](int u, const Pack8& w) {
+    uint2 c;
+    c.x = Code<kFp8>::four(p.value(w.w[0] & 0xffffu), p.value(w.w[0] >> 16), p.value(w.w[1] & 0xffffu), p.value(w.w[1] >> 16));
+    c.y = Code<kFp8>::four(p.value(w.w[2] & 0xffffu), p.value(w.w[2] >> 16), p.value(w.w[3] & 0xffffu), p.value(w.w[3] >> 16));
+    *reinterpret_cast<uint2*>(cache + (size_t)run.off * D + 8 * u) = c;
+  };
+#pragma unroll
+  for (int i = 0; i < kKept; ++i)
+    if (tid + i * kThreads < units) write(tid + i * kThreads, kept[i]);
+  for (int u = tid + kKept * kThreads; u < units; u += kThreads) write(u, read(u));
+  if (p.grows) {
+    for (int u = tid; u < run.off * (D / 16); u += kThreads) {
+      uint4 w = *reinterpret_cast<const uint4*>(cache + (size_t)u * 16);
+      w.x = moved<kFp8>(w.x, p.ratio), w.y = moved<kFp8>(w.y, p.ratio), w.z = moved<kFp8>(w.z, p.ratio), w.w = moved<kFp8>(w.w, p.ratio);
+      *reinterpret_cast<uint4*>(cache + (size_t)u * 16) = w;
     }
+  }
+}
+
+// A run's values: two dimensions of 8 positions a thread and unit, since a
+// dimension's positions are contiguous in the cache. No byte has two writers:
+// whole new units and changed old ones are stored as 8 bytes, a few new
+// positions as bytes.
+template <int D, bool kFp8, int kTeam>
+__device__ __forceinline__ void append_values(const Append& a, AppendShared& sh, int h, const Run& run, int tid) {
+  constexpr int kPer = D / 2, kThreads = kTeam * kWave, kKept = 2;
+  uint8_t* const cache = a.cache[1] + (((size_t)run.id * a.kv + h) * (size_t)D << a.shift);
+  float* const scale_at = a.scales[1] + (size_t)run.id * a.kv + h;
+  const int64_t stride = a.stride[1];
+  const uint16_t* const x = a.x[1] + (size_t)run.r0 * stride + (size_t)h * D;
+  const int off = run.off, to = run.off + run.len, b0 = off >> 3, units = (((to + 7) >> 3) - b0) * kPer;
+  struct Words {
+    uint32_t w[8];
+  };
+  // (positions outside the run repeat its first or last row: no larger, and not written)
+  const auto read = [&](int u) {
+    const int d = 2 * (u % kPer), r = 8 * (b0 + u / kPer) - off;
+    Words w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w.w[i] = *reinterpret_cast<const uint32_t*>(x + min(max(r + i, 0), run.len - 1) * stride + d);
+    return w;
+  };
+  Words kept[kKept];
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) kept[i] = read(min(tid + i * kThreads, units - 1));
+  const float old = off > 0 ? *scale_at : 0.0f;
+  uint32_t largest = 0;
+#pragma unroll
+  for (int i = 0; i < kKept; ++i)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) largest = largest_of(kept[i].w[k], largest);
+  for (int u = tid + kKept * kThreads; u < units; u += kThreads) {
+    const Words w = read(u);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) largest = largest_of(w.w[k], largest);
+  }
+  const PageScale p = page_scale<kFp8, kTeam>(sh, tid, largest, old, off, scale_at);
+  const auto write = [&](int u, const Words& w) {
+    const int d = 2 * (u % kPer), p0 = 8 * (b0 + u / kPer);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      uint8_t* const at = cache + (((size_t)(d + k)) << a.shift) + p0;
-      uint32_t c[4];
+      uint8_t* const at = cache + ((size_t)(d + k) << a.shift) + p0;
+      uint32_t c[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 2; ++i) {
         float f[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = code_of(k ? w[4 * i + j] >> 16 : w[4 * i + j] & 0xffffu);
+        for (int j = 0; j < 4; ++j) f[j] = p.value(k ? w.w[4 * i + j] >> 16 : w.w[4 * i + j] & 0xffffu);
         c[i] = Code<kFp8>::four(f[0], f[1], f[2], f[3]);
       }
-      const bool whole = p0 >= off && p0 + 16 <= off + len;
-      if (!whole && grows && p0 < off) {  // old positions before `off`, perhaps new ones behind them
-        const uint4 o = *reinterpret_cast<const uint4*>(at);
-        const uint32_t was[4] = {o.x, o.y, o.z, o.w};
+      if (p0 >= off && p0 + 8 <= to) {
+        *reinterpret_cast<uint2*>(at) = uint2{c[0], c[1]};
+      } else if (p.grows && p0 < off) {  // old positions before `off`, the run's behind them
+        const uint2 was = *reinterpret_cast<const uint2*>(at);
+        const uint32_t o[2] = {was.x, was.y};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t m = moved(was[i]);
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t m = moved<kFp8>(o[i], p.ratio);
           uint32_t r = 0;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int pos = p0 + 4 * i + j;
-            const uint32_t from = pos < off ? m : pos < off + len ? c[i] : was[i];
-            r |= from & (0xffu << (8 * j));
+            r |= (pos < off ? m : pos < to ? c[i] : o[i]) & (0xffu << (8 * j));
           }
           c[i] = r;
         }
-      }
-      if (whole || (grows && p0 < off)) {
-        *reinterpret_cast<uint4*>(at) = uint4{c[0], c[1], c[2], c[3]};
+        *reinterpret_cast<uint2*>(at) = uint2{c[0], c[1]};
       } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (p0 + i >= off && p0 + i < off + len) at[i] = (uint8_t)(c[i / 4] >> (8 * (i % 4)));
+        for (int i = 0; i < 8; ++i)
+          if (p0 + i >= off && p0 + i < to) at[i] = (uint8_t)(c[i / 4] >> (8 * (i % 4)));
       }
     }
+  };
+#pragma unroll
+  for (int i = 0; i < kKept; ++i)
+    if (tid + i * kThreads < units) write(tid + i * kThreads, kept[i]);
+  for (int u = tid + kKept * kThreads; u < units; u += kThreads) write(u, read(u));
+  if (p.grows) {  // the units before the run's
+    for (int u = tid; u < b0 * D; u += kThreads) {
+      uint8_t* const at = cache + ((size_t)(u % D) << a.shift) + 8 * (u / D);
+      uint2 w = *reinterpret_cast<const uint2*>(at);
+      w.x = moved<kFp8>(w.x, p.ratio), w.y = moved<kFp8>(w.y, p.ratio);
+      *reinterpret_cast<uint2*>(at) = w;
+    }
   }
-  (void)page;
 }
 
 // A run is consecutive rows whose slots follow one another within one page;
 // each is handled whole, where it begins, so that its page's scale has one
-// writer. Block (c, h): the runs that begin in rows [chunk c, chunk (c + 1))
-// of KV head h; long runs by the whole block (two waves for the keys, two for
-// the values), short ones by a wave for each of the two.
+// writer. Block (c, h, k): the runs that begin in rows [chunk c, chunk (c +
+// 1)) of KV head h, keys (k = 0) or values; a long run by the block's four
+// waves, a short one by one of them.
 template <int D, bool kFp8>
 __global__ void __launch_bounds__(kAppendThreads) k_kv8_append(const Append a) {
   __shared__ AppendShared sh;
   const int h = blockIdx.y, w = wave_id(), l = lane_id(), page = 1 << a.shift;
   const int most = a.pages << a.shift;  // (the host checks that it is an int)
   const int c0 = blockIdx.x * a.chunk;
+  // lane l: the slot of row c0 - 1 + l
+  const int mine = c0 - 1 + l;
+  const int slot = mine >= 0 && mine < a.rows ? a.slots[mine] : -1;
+  const int before = __shfl_up(slot, 1, kWave);
+  const bool valid = slot >= 0 && slot < most;
+  const bool begins = valid && l >= 1 && l <= a.chunk && !((slot & (page - 1)) != 0 && before == slot - 1);
   int turn = 0;
-  for (int r0 = c0; r0 < min(c0 + a.chunk, a.rows); ++r0) {
-    const int slot = a.slots[r0];
-    if (slot < 0 || slot >= most) continue;
-    const int off = slot & (page - 1);
-    if (off != 0 && r0 > 0 && a.slots[r0 - 1] == slot - 1) continue;  // not where its run begins
-    int len = 1;
-    while (true) {
-      const int k = len + l;  // does row r0 + k continue the run?
-      const bool on = off + k < page && r0 + k < a.rows && a.slots[min(r0 + k, a.rows - 1)] == slot + k;
-      const uint64_t stop = ~__ballot(on);
-      if (stop) {
-        len += __builtin_ctzll(stop);
-        break;
+  for (uint64_t heads = __ballot(begins); heads; heads &= heads - 1) {
+    const int at = __builtin_ctzll(heads), first = __builtin_amdgcn_readlane(slot, at);
+    Run run;
+    run.r0 = c0 - 1 + at;
+    run.id = first >> a.shift;
+    run.off = first & (page - 1);
+    const uint64_t on = __ballot(l > at && slot == first + (l - at) && run.off + (l - at) < page);
+    run.len = 1 + __builtin_ctzll(~(on >> at >> 1));
+    if (at + run.len == kWave) {  // it may go on behind the rows that were looked at
+      while (true) {
+        const int k = run.len + l;
+        const bool more = run.off + k < page && run.r0 + k < a.rows && a.slots[min(run.r0 + k, a.rows - 1)] == first + k;
+        const uint64_t stop = ~__ballot(more);
+        run.len += stop ? __builtin_ctzll(stop) : kWave;
+        if (stop) break;
       }
-      len += kWave;
     }
-    const int id = slot >> a.shift;
-    if (len >= 8) {
-      append_run<D, kFp8, 2>(a, sh, w >> 1, w & 1, h, id, off, r0, len);
+    if (run.len >= 8) {
+      if (blockIdx.z == 0) append_keys<D, kFp8, 4>(a, sh, h, run, threadIdx.x);
+      else append_values<D, kFp8, 4>(a, sh, h, run, threadIdx.x);
     } else {
-      if ((turn & 1) == (w >> 1)) append_run<D, kFp8, 1>(a, sh, w & 1, 0, h, id, off, r0, len);
+      if ((turn & 3) == w) {
+        if (blockIdx.z == 0) append_keys<D, kFp8, 1>(a, sh, h, run, l);
+        else append_values<D, kFp8, 1>(a, sh, h, run, l);
+      }
       ++turn;
     }
   }
@@ -1376,6 +1526,13 @@ size_t part_floats(const Splits& s, int64_t rows, int64_t heads, int64_t dim) {
   return most == 1 ? 0 : (size_t)(most * rows * heads * (dim + 2));
 }
 
+template <int kThreads, int kEach>
+void plan(const lfm25_kv8_plan_call& c, int shift, hipStream_t stream) {
+  hipLaunchKernelGGL((k_kv8_plan<kThreads, kEach>), dim3(1), dim3(kThreads), sizeof(PlanShared<kThreads * kEach>), stream, c.past,
+                     c.counts, c.requests, c.block_table, c.width, c.free_pages, c.ring, c.cursor, c.row_starts, c.slots, c.rows,
+                     c.next_cursor, c.status, shift);
+}
+
 template <int D, bool kFp8>
 int attend(const Attend& a, const Splits& s, hipStream_t stream) {
   const int64_t narrow = (int64_t)a.requests * a.kv * a.narrow_splits;
@@ -1397,50 +1554,60 @@ int attend(const Attend& a, const Splits& s, hipStream_t stream) {
 
 using namespace lfm25;
 
-extern "C" int lfm25_kv8_plan(const int32_t* past, const int32_t* counts, int32_t requests, int32_t* block_table, int32_t width,
-                              int32_t* free_pages, int32_t ring, const int64_t* cursor, int32_t* row_starts, int32_t* slots,
-                              int32_t rows, int64_t* next_cursor, int32_t* status, int32_t page, lfm25_stream_t stream) {
-  LFM25_REQUIRE(past && counts && block_table && free_pages && cursor && row_starts && slots && next_cursor && status,
+extern "C" int lfm25_kv8_plan(const lfm25_kv8_plan_call* call, lfm25_stream_t stream) {
+  LFM25_REQUIRE(call, "lfm25_kv8_plan: null pointer");
+  const lfm25_kv8_plan_call& c = *call;
+  LFM25_REQUIRE(c.past && c.counts && c.block_table && c.free_pages && c.cursor && c.row_starts && c.slots && c.next_cursor && c.status,
                 "lfm25_kv8_plan: null pointer");
-  LFM25_REQUIRE(page_shift(page) >= 0, "lfm25_kv8_plan: page must be 16, 32, 64, 128 or 256");
-  LFM25_REQUIRE(requests >= 1 && requests <= kMaxRequests, "lfm25_kv8_plan: requests must be in [1, %d]", kMaxRequests);
-  LFM25_REQUIRE(width >= 1 && (int64_t)width * page <= INT32_MAX, "lfm25_kv8_plan: width * page must be in [1, 2^31)");
-  LFM25_REQUIRE(ring >= 1 && rows >= 1, "lfm25_kv8_plan: an empty ring or no rows");
-  LFM25_REQUIRE(aligned4(past) && aligned4(counts) && aligned4(block_table) && aligned4(free_pages) && aligned4(row_starts) &&
-                    aligned4(slots) && aligned4(status) && aligned8(cursor) && aligned8(next_cursor),
+  LFM25_REQUIRE(page_shift(c.page) >= 0, "lfm25_kv8_plan: page must be 16, 32, 64, 128 or 256");
+  LFM25_REQUIRE(c.requests >= 1 && c.requests <= kMaxRequests, "lfm25_kv8_plan: requests must be in [1, %d]", kMaxRequests);
+  LFM25_REQUIRE(c.width >= 1 && (int64_t)c.width * c.page <= INT32_MAX, "lfm25_kv8_plan: width * page must be in [1, 2^31)");
+  LFM25_REQUIRE(c.ring >= 1 && c.rows >= 1, "lfm25_kv8_plan: an empty ring or no rows");
+  LFM25_REQUIRE(aligned4(c.past) && aligned4(c.counts) && aligned4(c.block_table) && aligned4(c.free_pages) && aligned4(c.row_starts) &&
+                    aligned4(c.slots) && aligned4(c.status) && aligned8(c.cursor) && aligned8(c.next_cursor),
                 "lfm25_kv8_plan: misaligned pointer");
-  hipLaunchKernelGGL(k_kv8_plan, dim3(1), dim3(kPlanThreads), 0, stream, past, counts, requests, block_table, width, free_pages, ring,
-                     cursor, row_starts, slots, rows, next_cursor, status, page_shift(page));
+  const int shift = page_shift(c.page);
+  // small passes with few waves to wait for one another, large ones with as
+  // many threads as a block has
+  if (c.requests <= 64 && c.rows <= 256) plan<64, 1>(c, shift, stream);
+  else if (c.requests <= 256 && c.rows <= 1024) plan<256, 1>(c, shift, stream);
+  else if (c.requests <= 1024) plan<1024, 1>(c, shift, stream);
+  else plan<1024, 4>(c, shift, stream);
+  if (c.rows > kPlanRows)
+    hipLaunchKernelGGL(k_kv8_slots, dim3((unsigned)((c.rows + (int64_t)kSlotThreads - 1) / kSlotThreads)), dim3(kSlotThreads), 0, stream,
+                       c.past, c.requests, c.block_table, c.width, c.row_starts, c.status, c.slots, c.rows, shift);
   return check_launch("lfm25_kv8_plan");
 }
 
-extern "C" int lfm25_kv8_append(const uint16_t* keys, int64_t key_stride, const uint16_t* values, int64_t value_stride,
-                                const int32_t* slots, int32_t rows, void* key_cache, void* value_cache, float* key_scales,
-                                float* value_scales, int32_t pages, int32_t page, int32_t kv_heads, int32_t head_dim,
-                                int32_t format, lfm25_stream_t stream) {
-  LFM25_REQUIRE(keys && values && slots && key_cache && value_cache && key_scales && value_scales, "lfm25_kv8_append: null pointer");
-  if (!cache_shape(pages, page, kv_heads, head_dim, format)) return LFM25_EINVAL;
-  LFM25_REQUIRE(rows >= 1, "lfm25_kv8_append: no rows");
-  const int64_t row = (int64_t)kv_heads * head_dim;
-  LFM25_REQUIRE(key_stride >= row && value_stride >= row && key_stride % 8 == 0 && value_stride % 8 == 0,
+extern "C" int lfm25_kv8_append(const lfm25_kv8_append_call* call, lfm25_stream_t stream) {
+  LFM25_REQUIRE(call, "lfm25_kv8_append: null pointer");
+  const lfm25_kv8_append_call& c = *call;
+  LFM25_REQUIRE(c.keys && c.values && c.slots && c.key_cache && c.value_cache && c.key_scales && c.value_scales,
+                "lfm25_kv8_append: null pointer");
+  if (!cache_shape(c.pages, c.page, c.kv_heads, c.head_dim, c.format)) return LFM25_EINVAL;
+  LFM25_REQUIRE(c.rows >= 1, "lfm25_kv8_append: no rows");
+  const int64_t row = (int64_t)c.kv_heads * c.head_dim;
+  LFM25_REQUIRE(c.key_stride >= row && c.value_stride >= row && c.key_stride % 8 == 0 && c.value_stride % 8 == 0,
                 "lfm25_kv8_append: row strides must be multiples of 8 of at least kv_heads * head_dim");
-  LFM25_REQUIRE(aligned16(keys) && aligned16(values) && aligned16(key_cache) && aligned16(value_cache),
+  LFM25_REQUIRE(aligned16(c.keys) && aligned16(c.values) && aligned16(c.key_cache) && aligned16(c.value_cache),
                 "lfm25_kv8_append: keys, values and caches must be 16-byte aligned");
-  LFM25_REQUIRE(aligned4(slots) && aligned4(key_scales) && aligned4(value_scales), "lfm25_kv8_append: misaligned pointer");
+  LFM25_REQUIRE(aligned4(c.slots) && aligned4(c.key_scales) && aligned4(c.value_scales), "lfm25_kv8_append: misaligned pointer");
   Append a{};
-  a.x[0] = keys, a.x[1] = values;
-  a.stride[0] = key_stride, a.stride[1] = value_stride;
-  a.cache[0] = static_cast<uint8_t*>(key_cache), a.cache[1] = static_cast<uint8_t*>(value_cache);
-  a.scales[0] = key_scales, a.scales[1] = value_scales;
-  a.slots = slots;
-  a.rows = rows, a.kv = kv_heads, a.pages = pages, a.shift = page_shift(page);
-  a.chunk = rows <= 512 ? 2 : 8;
-  const dim3 grid((unsigned)((rows + a.chunk - 1) / a.chunk), (unsigned)kv_heads), block(kAppendThreads);
-  if (head_dim == 64) {
-    if (format == LFM25_KV8_FP8) hipLaunchKernelGGL((k_kv8_append<64, true>), grid, block, 0, stream, a);
+  a.x[0] = c.keys, a.x[1] = c.values;
+  a.stride[0] = c.key_stride, a.stride[1] = c.value_stride;
+  a.cache[0] = static_cast<uint8_t*>(c.key_cache), a.cache[1] = static_cast<uint8_t*>(c.value_cache);
+  a.scales[0] = c.key_scales, a.scales[1] = c.value_scales;
+  a.slots = c.slots;
+  a.rows = c.rows, a.kv = c.kv_heads, a.pages = c.pages, a.shift = page_shift(c.page);
+  // few rows: a single token of a request for each wave; many: blocks for a
+  // quarter of a page of 64 or less, most of which find no run to begin
+  a.chunk = c.rows <= 512 ? 4 : 16;
+  const dim3 grid((unsigned)((c.rows + (int64_t)a.chunk - 1) / a.chunk), (unsigned)c.kv_heads, 2), block(kAppendThreads);
+  if (c.head_dim == 64) {
+    if (c.format == LFM25_KV8_FP8) hipLaunchKernelGGL((k_kv8_append<64, true>), grid, block, 0, stream, a);
     else hipLaunchKernelGGL((k_kv8_append<64, false>), grid, block, 0, stream, a);
   } else {
-    if (format == LFM25_KV8_FP8) hipLaunchKernelGGL((k_kv8_append<128, true>), grid, block, 0, stream, a);
+    if (c.format == LFM25_KV8_FP8) hipLaunchKernelGGL((k_kv8_append<128, true>), grid, block, 0, stream, a);
     else hipLaunchKernelGGL((k_kv8_append<128, false>), grid, block, 0, stream, a);
   }
   return check_launch("lfm25_kv8_append");
@@ -1465,42 +1632,42 @@ extern "C" size_t lfm25_kv8_attention_workspace_bytes(int32_t rows, int32_t head
   return 4 * part_floats(s, rows, heads, head_dim);
 }
 
-extern "C" int lfm25_kv8_attention(const uint16_t* query, int64_t query_stride, const void* key_cache, const void* value_cache,
-                                   const float* key_scales, const float* value_scales, const int32_t* block_table, int32_t width,
-                                   const int32_t* past, const int32_t* row_starts, int32_t requests, uint16_t* output, int32_t rows,
-                                   int32_t heads, int32_t max_rows, float scale, int32_t pages, int32_t page, int32_t kv_heads,
-                                   int32_t head_dim, int32_t format, int32_t* status, void* workspace, lfm25_stream_t stream) {
-  LFM25_REQUIRE(query && key_cache && value_cache && key_scales && value_scales && block_table && past && row_starts && output,
+extern "C" int lfm25_kv8_attention(const lfm25_kv8_attention_call* call, lfm25_stream_t stream) {
+  LFM25_REQUIRE(call, "lfm25_kv8_attention: null pointer");
+  const lfm25_kv8_attention_call& c = *call;
+  LFM25_REQUIRE(c.query && c.key_cache && c.value_cache && c.key_scales && c.value_scales && c.block_table && c.past && c.row_starts &&
+                    c.output,
                 "lfm25_kv8_attention: null pointer");
-  if (!cache_shape(pages, page, kv_heads, head_dim, format)) return LFM25_EINVAL;
-  if (!attend_shape(rows, heads, kv_heads, requests, max_rows, width, page)) return LFM25_EINVAL;
-  LFM25_REQUIRE(query_stride >= (int64_t)heads * head_dim && query_stride % 8 == 0,
+  if (!cache_shape(c.pages, c.page, c.kv_heads, c.head_dim, c.format)) return LFM25_EINVAL;
+  if (!attend_shape(c.rows, c.heads, c.kv_heads, c.requests, c.max_rows, c.width, c.page)) return LFM25_EINVAL;
+  LFM25_REQUIRE(c.query_stride >= (int64_t)c.heads * c.head_dim && c.query_stride % 8 == 0,
                 "lfm25_kv8_attention: the query's row stride must be a multiple of 8 of at least heads * head_dim");
-  LFM25_REQUIRE(aligned16(query) && aligned16(key_cache) && aligned16(value_cache) && aligned16(output),
+  LFM25_REQUIRE(aligned16(c.query) && aligned16(c.key_cache) && aligned16(c.value_cache) && aligned16(c.output),
                 "lfm25_kv8_attention: query, output and caches must be 16-byte aligned");
-  LFM25_REQUIRE(aligned4(key_scales) && aligned4(value_scales) && aligned4(block_table) && aligned4(past) && aligned4(row_starts) &&
-                    aligned4(status),
+  LFM25_REQUIRE(aligned4(c.key_scales) && aligned4(c.value_scales) && aligned4(c.block_table) && aligned4(c.past) &&
+                    aligned4(c.row_starts) && aligned4(c.status),
                 "lfm25_kv8_attention: misaligned pointer");
-  LFM25_REQUIRE(std::isfinite(scale) && scale >= 0.0f, "lfm25_kv8_attention: scale must be finite and not negative");
-  max_rows = std::min(max_rows, rows);
-  const Splits s = splits_for(rows, requests, kv_heads, heads / kv_heads, max_rows, width, page);
-  const size_t floats = part_floats(s, rows, heads, head_dim);
-  LFM25_REQUIRE(floats == 0 || (workspace != nullptr && aligned16(workspace)),
+  LFM25_REQUIRE(std::isfinite(c.scale) && c.scale >= 0.0f, "lfm25_kv8_attention: scale must be finite and not negative");
+  LFM25_REQUIRE(c.reserved == 0, "lfm25_kv8_attention: reserved must be 0");
+  const int group = c.heads / c.kv_heads, max_rows = std::min(c.max_rows, c.rows);
+  const Splits s = splits_for(c.rows, c.requests, c.kv_heads, group, max_rows, c.width, c.page);
+  const size_t floats = part_floats(s, c.rows, c.heads, c.head_dim);
+  LFM25_REQUIRE(floats == 0 || (c.workspace != nullptr && aligned16(c.workspace)),
                 "lfm25_kv8_attention: needs a 16-byte aligned workspace of lfm25_kv8_attention_workspace_bytes()");
   Attend a{};
-  a.q = query, a.q_stride = query_stride;
-  a.k = static_cast<const uint8_t*>(key_cache), a.v = static_cast<const uint8_t*>(value_cache);
-  a.ks = key_scales, a.vs = value_scales;
-  a.table = block_table, a.past = past, a.starts = row_starts;
-  a.out = output;
-  a.part = static_cast<float*>(workspace);
-  a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)std::max(s.narrow, s.wide) * rows * heads * head_dim);
-  a.status = status;
-  a.width = width, a.rows = rows, a.kv = kv_heads, a.group = heads / kv_heads, a.pages = pages, a.shift = page_shift(page);
-  a.requests = requests, a.max_rows = max_rows;
+  a.q = c.query, a.q_stride = c.query_stride;
+  a.k = static_cast<const uint8_t*>(c.key_cache), a.v = static_cast<const uint8_t*>(c.value_cache);
+  a.ks = c.key_scales, a.vs = c.value_scales;
+  a.table = c.block_table, a.past = c.past, a.starts = c.row_starts;
+  a.out = c.output;
+  a.part = static_cast<float*>(c.workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)std::max(s.narrow, s.wide) * c.rows * c.heads * c.head_dim);
+  a.status = c.status;
+  a.width = c.width, a.rows = c.rows, a.kv = c.kv_heads, a.group = group, a.pages = c.pages, a.shift = page_shift(c.page);
+  a.requests = c.requests, a.max_rows = max_rows;
   a.narrow_splits = s.narrow, a.wide_splits = s.wide;
-  a.wide_blocks = (int)(s.wide_tiles * kv_heads * s.wide);
-  a.scale = scale * 1.4426950408889634f;
-  if (head_dim == 64) return format == LFM25_KV8_FP8 ? attend<64, true>(a, s, stream) : attend<64, false>(a, s, stream);
-  return format == LFM25_KV8_FP8 ? attend<128, true>(a, s, stream) : attend<128, false>(a, s, stream);
+  a.wide_blocks = (int)(s.wide_tiles * c.kv_heads * s.wide);
+  a.scale = c.scale * 1.4426950408889634f;
+  if (c.head_dim == 64) return c.format == LFM25_KV8_FP8 ? attend<64, true>(a, s, stream) : attend<64, false>(a, s, stream);
+  return c.format == LFM25_KV8_FP8 ? attend<128, true>(a, s, stream) : attend<128, false>(a, s, stream);
 }

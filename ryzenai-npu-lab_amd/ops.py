@@ -12,6 +12,9 @@ without waiting; NPU-only knobs such as n_cores are validated and ignored.
 
 from __future__ import annotations
 
+import functools
+import struct
+
 import torch
 
 from . import _lib
@@ -542,11 +545,28 @@ def bf16_f32_matmul(input0, input1, output, *, M: int, K: int, N: int, n_cores: 
 # kv8_plan, then per layer kv8_append and kv8_attention (lfm25_kv8_* in
 # include/lfm25_hip.h has the definitions). Nothing here waits for the GPU,
 # and all of it may be captured into a graph.
+#
+# These calls are short, so their checks are one expression each (a tensor's
+# attribute costs 0.07 us, a call 0.1), and the arguments go over as one packed
+# structure (0.5 us; 24 separate ones take ctypes 2.0): 12.5 -> 7 us a call.
+# Where the expression is false, the checks one by one name what is wrong.
 
 KV8_LENGTH, KV8_TABLE, KV8_POOL, KV8_ROWS = 1, 2, 4, 8  # kv8_plan's status
 KV8_BAD_PAGE, KV8_BAD_ROWS = 1, 2                       # kv8_attention's status bits
 _KV8_FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
-_KV8_PAGES = (16, 32, 64, 128, 256)
+_KV8_PAGES = frozenset((16, 32, 64, 128, 256))
+_KV8_MAX_REQUESTS = 4096
+_BF16, _F32, _INT32, _INT64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
+
+_PLAN = struct.Struct("@9P5i")
+_APPEND = struct.Struct("@7P2q6i")
+_ATTEND = struct.Struct("@11Pq11if")
+
+
+if hasattr(torch._C, "_cuda_getDevice"):
+    _device = torch._C._cuda_getDevice
+else:  # a torch without this private name
+    _device = torch.cuda.current_device
 
 
 def _here(*tensors) -> None:
@@ -557,30 +577,24 @@ def _here(*tensors) -> None:
             raise ValueError(f"tensors must be on the current device (cuda:{device}), got {t.device}")
 
 
-def _kv8_rows(t, name: str, heads: int, dim: int, rows: int) -> int:
-    """Address of BF16 rows [rows, heads, dim] whose rows may be apart."""
+def _kv8_rows(t, name: str, heads: int, dim: int, rows: int) -> None:
+    """BF16 rows [rows, heads, dim], which may be apart."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a GPU tensor")
-    if t.dtype != torch.bfloat16:
-        raise ValueError(f"{name} must be {torch.bfloat16}, got {t.dtype}")
+    if t.dtype != _BF16:
+        raise ValueError(f"{name} must be {_BF16}, got {t.dtype}")
     if t.shape != (rows, heads, dim):
         raise ValueError(f"{name} must be [{rows}, {heads}, {dim}], got {list(t.shape)}")
     s = t.stride()
     if s[2] != 1 or (heads > 1 and s[1] != dim):
         raise ValueError(f"{name}: a row's heads must be contiguous")
-    return t.data_ptr()
-
-
-def _kv8_stride(t) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
 
 
 def _kv8_cache(key_cache, value_cache, key_scales, value_scales):
-    """(pages, page, kv_heads, dim, format) of a cache's four tensors."""
+    """(pages, kv_heads, page, dim) of a cache's four tensors."""
     if not isinstance(key_cache, torch.Tensor) or key_cache.dim() != 4:
         raise ValueError("key_cache must be [pages, kv_heads, page, dim]")
-    form = _KV8_FORMATS.get(key_cache.dtype)
-    if form is None:
+    if key_cache.dtype not in _KV8_FORMATS:
         raise ValueError(f"key_cache must be torch.int8 or torch.float8_e4m3fn, got {key_cache.dtype}")
     pages, kv, page, dim = key_cache.shape
     if page not in _KV8_PAGES or dim not in (64, 128):
@@ -589,11 +603,39 @@ def _kv8_cache(key_cache, value_cache, key_scales, value_scales):
     _check(value_cache, "value_cache", key_cache.dtype)
     if value_cache.shape != (pages, kv, dim, page):
         raise ValueError(f"value_cache must be [{pages}, {kv}, {dim}, {page}], got {list(value_cache.shape)}")
-    for t, name in ((key_scales, "key_scales"), (value_scales, "value_scales")):
-        _f32(t, name)
-        if t.shape != (pages, kv):
-            raise ValueError(f"{name} must be [{pages}, {kv}], got {list(t.shape)}")
-    return pages, page, kv, dim, form
+    _f32(key_scales, "key_scales", pages * kv)
+    _f32(value_scales, "value_scales", pages * kv)
+    return pages, kv, page, dim
+
+
+def _kv8_table(block_table, requests: int) -> None:
+    _i32(block_table, "block_table")
+    if block_table.dim() != 2 or block_table.shape[0] != requests or block_table.shape[1] < 1:
+        raise ValueError(f"block_table must be [{requests}, width]")
+
+
+def _kv8_requests(past) -> int:
+    if isinstance(past, torch.Tensor) and not 1 <= past.numel() <= _KV8_MAX_REQUESTS:
+        raise ValueError(f"past must hold 1 to {_KV8_MAX_REQUESTS} lengths")
+    _i32(past, "past")
+    return past.numel()
+
+
+def _kv8_plan_check(past, counts, block_table, free_pages, cursor, row_starts, slots, next_cursor, status, page) -> None:
+    if page not in _KV8_PAGES:
+        raise ValueError("page must be 16, 32, 64, 128 or 256")
+    n = _kv8_requests(past)
+    _i32(counts, "counts", n)
+    _kv8_table(block_table, n)
+    _i32(free_pages, "free_pages")
+    _check(cursor, "cursor", _INT64, 2)
+    _i32(row_starts, "row_starts", n + 1)
+    _i32(slots, "slots")
+    _check(next_cursor, "next_cursor", _INT64, 2)
+    _i32(status, "status", n)
+    if free_pages.numel() < 1 or slots.numel() < 1:
+        raise ValueError("free_pages and slots must not be empty")
+    _here(past, counts, block_table, free_pages, cursor, row_starts, slots, next_cursor, status)
 
 
 def kv8_plan(past, counts, block_table, free_pages, cursor, row_starts, slots, next_cursor, status, *, page: int) -> None:
@@ -606,28 +648,38 @@ def kv8_plan(past, counts, block_table, free_pages, cursor, row_starts, slots, n
     [requests + 1], slots int32 [rows] (-1: a refused request's row, or behind
     the last), next_cursor int64 [2] (may be cursor), status int32 [requests]
     (0, or KV8_LENGTH / KV8_TABLE / KV8_POOL / KV8_ROWS)."""
-    if page not in _KV8_PAGES:
-        raise ValueError("page must be 16, 32, 64, 128 or 256")
-    n = past.numel() if isinstance(past, torch.Tensor) else 0
-    if not 1 <= n <= 4096:
-        raise ValueError("past must be a tensor of 1 to 4096 lengths")
-    _i32(past, "past")
-    _i32(counts, "counts", n)
-    _i32(block_table, "block_table")
-    if block_table.dim() != 2 or block_table.shape[0] != n or block_table.shape[1] < 1:
-        raise ValueError(f"block_table must be [{n}, width]")
-    _i32(free_pages, "free_pages")
-    _check(cursor, "cursor", torch.int64, 2)
-    _i32(row_starts, "row_starts", n + 1)
+    try:
+        n, ring, rows, here = past.numel(), free_pages.numel(), slots.numel(), past.get_device()
+        wide = block_table.shape
+        fine = (page in _KV8_PAGES and 1 <= n <= _KV8_MAX_REQUESTS and ring > 0 and rows > 0 and len(wide) == 2
+                and wide[0] == n and wide[1] > 0 and here >= 0
+                and past.dtype is _INT32 and counts.dtype is _INT32 and block_table.dtype is _INT32
+                and free_pages.dtype is _INT32 and row_starts.dtype is _INT32 and slots.dtype is _INT32
+                and status.dtype is _INT32 and cursor.dtype is _INT64 and next_cursor.dtype is _INT64
+                and counts.numel() == n and row_starts.numel() == n + 1 and status.numel() == n
+                and cursor.numel() == 2 and next_cursor.numel() == 2
+                and past.is_contiguous() and counts.is_contiguous() and block_table.is_contiguous()
+                and free_pages.is_contiguous() and row_starts.is_contiguous() and slots.is_contiguous()
+                and status.is_contiguous() and cursor.is_contiguous() and next_cursor.is_contiguous()
+                and here == counts.get_device() == block_table.get_device() == free_pages.get_device()
+                == row_starts.get_device() == slots.get_device() == status.get_device() == cursor.get_device()
+                == next_cursor.get_device() and here == _device())
+    except AttributeError:
+        fine = False
+    if not fine:
+        _kv8_plan_check(past, counts, block_table, free_pages, cursor, row_starts, slots, next_cursor, status, page)
+    _lib.call("lfm25_kv8_plan", _PLAN.pack(
+        past.data_ptr(), counts.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), cursor.data_ptr(),
+        row_starts.data_ptr(), slots.data_ptr(), next_cursor.data_ptr(), status.data_ptr(), n, wide[1], ring, rows, page),
+        _stream())
+
+
+def _kv8_append_check(keys, values, slots, key_cache, value_cache, key_scales, value_scales) -> None:
+    _, kv, _, dim = _kv8_cache(key_cache, value_cache, key_scales, value_scales)
     _i32(slots, "slots")
-    _check(next_cursor, "next_cursor", torch.int64, 2)
-    _i32(status, "status", n)
-    if free_pages.numel() < 1 or slots.numel() < 1:
-        raise ValueError("free_pages and slots must not be empty")
-    _here(past, counts, block_table, free_pages, cursor, row_starts, slots, next_cursor, status)
-    _lib.call("lfm25_kv8_plan", past.data_ptr(), counts.data_ptr(), n, block_table.data_ptr(), block_table.shape[1],
-              free_pages.data_ptr(), free_pages.numel(), cursor.data_ptr(), row_starts.data_ptr(), slots.data_ptr(),
-              slots.numel(), next_cursor.data_ptr(), status.data_ptr(), page, _stream())
+    _kv8_rows(keys, "keys", kv, dim, slots.numel())
+    _kv8_rows(values, "values", kv, dim, slots.numel())
+    _here(keys, values, slots, key_cache, value_cache, key_scales, value_scales)
 
 
 def kv8_append(keys, values, slots, key_cache, value_cache, key_scales, value_scales) -> None:
@@ -637,15 +689,57 @@ def kv8_append(keys, values, slots, key_cache, value_cache, key_scales, value_sc
     row out). Written in place: key_cache [pages, kv_heads, page, dim] and
     value_cache [pages, kv_heads, dim, page] in torch.int8 or
     torch.float8_e4m3fn, key_scales and value_scales FP32 [pages, kv_heads]."""
-    pages, page, kv, dim, form = _kv8_cache(key_cache, value_cache, key_scales, value_scales)
-    _i32(slots, "slots")
-    rows = slots.numel()
-    k, v = _kv8_rows(keys, "keys", kv, dim, rows), _kv8_rows(values, "values", kv, dim, rows)
+    try:
+        pages, kv, page, dim = key_cache.shape
+        rows, here, code = slots.numel(), slots.get_device(), key_cache.dtype
+        ks, vs = keys.stride(), values.stride()
+        fine = (here >= 0 and code in _KV8_FORMATS and value_cache.dtype is code and page in _KV8_PAGES
+                and (dim == 64 or dim == 128) and value_cache.shape == (pages, kv, dim, page)
+                and keys.shape == values.shape == (rows, kv, dim) and ks[2] == vs[2] == 1
+                and (kv == 1 or ks[1] == vs[1] == dim)
+                and keys.dtype is _BF16 and values.dtype is _BF16 and slots.dtype is _INT32
+                and key_scales.dtype is _F32 and value_scales.dtype is _F32
+                and key_scales.numel() == value_scales.numel() == pages * kv
+                and slots.is_contiguous() and key_cache.is_contiguous() and value_cache.is_contiguous()
+                and key_scales.is_contiguous() and value_scales.is_contiguous()
+                and here == keys.get_device() == values.get_device() == key_cache.get_device()
+                == value_cache.get_device() == key_scales.get_device() == value_scales.get_device() and here == _device())
+    except (AttributeError, ValueError, IndexError):
+        fine = False
+    if not fine:
+        _kv8_append_check(keys, values, slots, key_cache, value_cache, key_scales, value_scales)
     if rows == 0:
         return
-    _here(keys, values, slots, key_cache, value_cache, key_scales, value_scales)
-    _lib.call("lfm25_kv8_append", k, _kv8_stride(keys), v, _kv8_stride(values), slots.data_ptr(), rows, key_cache.data_ptr(),
-              value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), pages, page, kv, dim, form, _stream())
+    _lib.call("lfm25_kv8_append", _APPEND.pack(
+        keys.data_ptr(), values.data_ptr(), slots.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+        key_scales.data_ptr(), value_scales.data_ptr(), ks[0] if rows > 1 else kv * dim, vs[0] if rows > 1 else kv * dim,
+        rows, pages, page, kv, dim, _KV8_FORMATS[code]), _stream())
+
+
+@functools.lru_cache(maxsize=256)
+def _kv8_workspace_bytes(*sizes: int) -> int:
+    return int(_lib.load().lfm25_kv8_attention_workspace_bytes(*sizes))
+
+
+def _kv8_attention_check(query, key_cache, value_cache, key_scales, value_scales, block_table, past, row_starts, output,
+                         status, max_rows, scale) -> None:
+    _, kv, _, dim = _kv8_cache(key_cache, value_cache, key_scales, value_scales)
+    _bf(output, "output")
+    if output.dim() != 3 or output.shape[2] != dim or output.shape[1] % kv or not 1 <= output.shape[1] // kv <= 16:
+        raise ValueError(f"output must be [rows, heads, {dim}] with heads a multiple (1 to 16) of {kv}")
+    _kv8_rows(query, "query", output.shape[1], dim, output.shape[0])
+    n = _kv8_requests(past)
+    _i32(row_starts, "row_starts", n + 1)
+    _kv8_table(block_table, n)
+    if max_rows < 1:
+        raise ValueError("max_rows must be positive")
+    if not 0.0 <= scale < float("inf"):
+        raise ValueError("scale must be finite and not negative")
+    tensors = [query, key_cache, value_cache, key_scales, value_scales, block_table, past, row_starts, output]
+    if status is not None:
+        _i32(status, "status", 1)
+        tensors.append(status)
+    _here(*tensors)
 
 
 def kv8_attention(query, key_cache, value_cache, key_scales, value_scales, block_table, past, row_starts, output, *,
@@ -659,35 +753,43 @@ def kv8_attention(query, key_cache, value_cache, key_scales, value_scales, block
     request. scale: of the scores, 1 / sqrt(dim) by default. Written: output
     BF16 [rows, heads, dim], contiguous; status (int32 [1], optional) gets bits
     KV8_BAD_PAGE / KV8_BAD_ROWS set."""
-    pages, page, kv, dim, form = _kv8_cache(key_cache, value_cache, key_scales, value_scales)
-    _bf(output, "output")
-    if output.dim() != 3 or output.shape[2] != dim or output.shape[1] % kv or not 1 <= output.shape[1] // kv <= 16:
-        raise ValueError(f"output must be [rows, heads, {dim}] with heads a multiple (1 to 16) of {kv}")
-    rows, heads = output.shape[:2]
-    q = _kv8_rows(query, "query", heads, dim, rows)
-    _i32(past, "past")
-    n = past.numel()
-    if not 1 <= n <= 4096:
-        raise ValueError("past must hold 1 to 4096 lengths")
-    _i32(row_starts, "row_starts", n + 1)
-    _i32(block_table, "block_table")
-    if block_table.dim() != 2 or block_table.shape[0] != n or block_table.shape[1] < 1:
-        raise ValueError(f"block_table must be [{n}, width]")
-    if max_rows < 1:
-        raise ValueError("max_rows must be positive")
-    scale = dim ** -0.5 if scale is None else scale
-    if not 0.0 <= scale < float("inf"):
-        raise ValueError("scale must be finite and not negative")
-    flags = 0 if status is None else _i32(status, "status", 1)
+    try:
+        pages, kv, page, dim = key_cache.shape
+        rows, heads, width = output.shape
+        n, here, code = past.numel(), past.get_device(), key_cache.dtype
+        qs, table = query.stride(), block_table.shape
+        if scale is None:
+            scale = dim ** -0.5
+        fine = (here >= 0 and width == dim and heads % kv == 0 and 1 <= heads // kv <= 16 and 1 <= n <= _KV8_MAX_REQUESTS
+                and max_rows >= 1 and 0.0 <= scale < 3.4e38 and code in _KV8_FORMATS and value_cache.dtype is code
+                and page in _KV8_PAGES and (dim == 64 or dim == 128) and value_cache.shape == (pages, kv, dim, page)
+                and query.shape == output.shape and qs[2] == 1 and (heads == 1 or qs[1] == dim)
+                and len(table) == 2 and table[0] == n and table[1] > 0
+                and query.dtype is _BF16 and output.dtype is _BF16 and block_table.dtype is _INT32 and past.dtype is _INT32
+                and row_starts.dtype is _INT32 and key_scales.dtype is _F32 and value_scales.dtype is _F32
+                and row_starts.numel() == n + 1 and key_scales.numel() == value_scales.numel() == pages * kv
+                and output.is_contiguous() and key_cache.is_contiguous() and value_cache.is_contiguous()
+                and key_scales.is_contiguous() and value_scales.is_contiguous() and block_table.is_contiguous()
+                and past.is_contiguous() and row_starts.is_contiguous()
+                and here == query.get_device() == key_cache.get_device() == value_cache.get_device()
+                == key_scales.get_device() == value_scales.get_device() == block_table.get_device()
+                == row_starts.get_device() == output.get_device() and here == _device()
+                and (status is None or (status.dtype is _INT32 and status.numel() == 1 and status.get_device() == here)))
+    except (AttributeError, ValueError, IndexError, TypeError, ZeroDivisionError):
+        fine = False
+    if not fine:
+        _kv8_attention_check(query, key_cache, value_cache, key_scales, value_scales, block_table, past, row_starts, output,
+                             status, max_rows, 0.0 if scale is None else scale)
     if rows == 0:
         return
-    _here(query, key_cache, value_cache, key_scales, value_scales, block_table, past, row_starts, output,
-          *(() if status is None else (status,)))
-    width = block_table.shape[1]
-    max_rows = min(max_rows, rows)
-    need = _lib.load().lfm25_kv8_attention_workspace_bytes(rows, heads, kv, dim, n, max_rows, width, page)
-    ws = torch.empty(need, dtype=torch.uint8, device=output.device) if need else None
-    _lib.call("lfm25_kv8_attention", q, _kv8_stride(query), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
-              value_scales.data_ptr(), block_table.data_ptr(), width, past.data_ptr(), row_starts.data_ptr(), n,
-              output.data_ptr(), rows, heads, max_rows, scale, pages, page, kv, dim, form, flags,
-              ws.data_ptr() if need else 0, _stream())
+    if max_rows > rows:
+        max_rows = rows
+    need = _kv8_workspace_bytes(rows, heads, kv, dim, n, max_rows, table[1], page)
+    # (the memory may go to another call of this stream once this one is queued)
+    workspace = torch.empty(need, dtype=torch.uint8, device=output.device) if need else None
+    _lib.call("lfm25_kv8_attention", _ATTEND.pack(
+        query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
+        block_table.data_ptr(), past.data_ptr(), row_starts.data_ptr(), output.data_ptr(),
+        0 if status is None else status.data_ptr(), workspace.data_ptr() if need else 0,
+        qs[0] if rows > 1 else heads * dim, table[1], n, rows, heads, max_rows, pages, page, kv, dim,
+        _KV8_FORMATS[code], 0, scale), _stream())

@@ -15,22 +15,46 @@ ODD = ctypes.c_void_p(4097)
 OFF8 = ctypes.c_void_p(4096 + 8)
 
 
+class PlanCall(ctypes.Structure):  # include/lfm25_hip.h
+    _fields_ = [(n, ctypes.c_void_p) for n in ("past", "counts", "table", "ring_at", "cursor", "starts", "slots", "next", "status")] + [
+        (n, ctypes.c_int32) for n in ("requests", "width", "ring", "rows", "page")]
+
+
+class AppendCall(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("keys", "values", "slots", "kc", "vc", "ksc", "vsc")] + [
+        (n, ctypes.c_int64) for n in ("ks", "vs")] + [(n, ctypes.c_int32) for n in ("rows", "pages", "page", "kv", "dim", "format")]
+
+
+class AttendCall(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("query", "kc", "vc", "ksc", "vsc", "table", "past", "starts", "out", "status", "ws")] + [
+        ("stride", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in (
+            "width", "requests", "rows", "heads", "max_rows", "pages", "page", "kv", "dim", "format", "reserved")] + [("scale", ctypes.c_float)]
+
+
 def plan_args(**change):
     a = dict(past=P, counts=P, requests=4, table=P, width=8, ring_at=P, ring=16, cursor=P, starts=P, slots=P, rows=4, next=P,
-             status=P, page=64, stream=None)
-    return list((a | change).values())
+             status=P, page=64)
+    return bytes(PlanCall(**(a | change))), None
 
 
 def append_args(**change):
-    a = dict(keys=P, ks=512, values=P, vs=512, slots=P, rows=4, kc=P, vc=P, ksc=P, vsc=P, pages=8, page=64, kv=8, dim=64,
-             format=0, stream=None)
-    return list((a | change).values())
+    a = dict(keys=P, ks=512, values=P, vs=512, slots=P, rows=4, kc=P, vc=P, ksc=P, vsc=P, pages=8, page=64, kv=8, dim=64, format=0)
+    return bytes(AppendCall(**(a | change))), None
 
 
 def attend_args(**change):
     a = dict(query=P, stride=1024, kc=P, vc=P, ksc=P, vsc=P, table=P, width=8, past=P, starts=P, requests=4, out=P, rows=4,
-             heads=16, max_rows=1, scale=0.125, pages=8, page=64, kv=8, dim=64, format=0, status=None, ws=None, stream=None)
-    return list((a | change).values())
+             heads=16, max_rows=1, scale=0.125, pages=8, page=64, kv=8, dim=64, format=0)
+    return bytes(AttendCall(**(a | change))), None
+
+
+def test_packed_calls_have_the_structures_sizes(lab):
+    for packed, call in ((lab.ops._PLAN, PlanCall), (lab.ops._APPEND, AppendCall), (lab.ops._ATTEND, AttendCall)):
+        # (struct leaves out the padding behind the last member)
+        assert 0 <= ctypes.sizeof(call) - packed.size < 8
+    lib = lab.load_library()
+    for f in (lib.lfm25_kv8_plan, lib.lfm25_kv8_append, lib.lfm25_kv8_attention):
+        assert f(None, None) == lab._lib.LFM25_EINVAL and b"null" in lib.lfm25_last_error()
 
 
 @pytest.mark.parametrize("change,message", [
@@ -62,7 +86,7 @@ def test_append_refuses(lab, change, message):
     (dict(rows=0), b"rows"), (dict(rows=1 << 28), b"rows"), (dict(requests=4097), b"requests"), (dict(max_rows=0), b"max_rows"),
     (dict(width=0), b"width"), (dict(width=1 << 26), b"width"), (dict(stride=1020), b"stride"), (dict(stride=1000), b"stride"),
     (dict(query=OFF8), b"aligned"), (dict(out=OFF8), b"aligned"), (dict(past=ODD), b"misaligned"), (dict(status=ODD), b"misaligned"),
-    (dict(scale=float("nan")), b"scale"), (dict(scale=-1.0), b"scale"), (dict(scale=float("inf")), b"scale"),
+    (dict(scale=float("nan")), b"scale"), (dict(scale=-1.0), b"scale"), (dict(scale=float("inf")), b"scale"), (dict(reserved=1), b"reserved"),
     (dict(width=64), b"workspace")])
 def test_attention_refuses(lab, change, message):
     lib = lab.load_library()
