@@ -251,17 +251,18 @@ __global__ void __launch_bounds__(kSlotThreads) k_kv8_slots(const int* __restric
 template <bool kFp8>
 struct Code;
 
-// int8: -127 .. 127, to the nearest, ties to even.
+// int8: -127 .. 127 (kMost), to the nearest, ties to even.
 template <>
 struct Code<false> {
-  static constexpr float kMost = 127.0f;
   static constexpr int kMostExponent = 6;     // 127 = 1.984375 * 2^6
   static constexpr uint32_t kMostMantissa = 0x7eu;  // the BF16 mantissa bits of 1.984375
-  __device__ static __forceinline__ uint32_t one(float v) {
-    return (uint32_t)(int)rintf(fminf(fmaxf(v, -kMost), kMost)) & 0xffu;
-  }
+  // (of values in -kMost .. kMost: 1.5 * 2^23 + v has the rounded v, modulo
+  // 256, in its last byte)
+  __device__ static __forceinline__ uint32_t rounded(float v) { return __float_as_uint(v + 0x1.8p23f); }
   __device__ static __forceinline__ uint32_t four(float a, float b, float c, float d) {
-    return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
+    const uint32_t lo = __builtin_amdgcn_perm(rounded(b), rounded(a), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(rounded(d), rounded(c), 0x0c0c0400u);
+    return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
   }
   __device__ static __forceinline__ void values(uint32_t w, float (&f)[4]) {
 #pragma unroll
@@ -277,19 +278,13 @@ struct Code<false> {
   }
 };
 
-// FP8 e4m3 (finite values up to 448), to the nearest, ties to even.
+// FP8 e4m3 (finite values up to kMost, 448), to the nearest, ties to even.
 template <>
 struct Code<true> {
-  static constexpr float kMost = 448.0f;
   static constexpr int kMostExponent = 8;     // 448 = 1.75 * 2^8
   static constexpr uint32_t kMostMantissa = 0x60u;  // the BF16 mantissa bits of 1.75
-  __device__ static __forceinline__ float in_range(float v) { return fminf(fmaxf(v, -kMost), kMost); }
-  __device__ static __forceinline__ uint32_t one(float v) {
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(in_range(v), 0.0f, 0, false) & 0xffu;
-  }
   __device__ static __forceinline__ uint32_t four(float a, float b, float c, float d) {
-    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(in_range(a), in_range(b), 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(in_range(c), in_range(d), lo, true);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
   }
   __device__ static __forceinline__ void values(uint32_t w, float (&f)[4]) {
     const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
@@ -342,13 +337,17 @@ __device__ __forceinline__ int wave_max_int(int v) {
              max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
 
-// The largest of a page's magnitude and the page's scale before and after.
+// A page's scale after a run came into it. value() is bf16 / scale (0 in a
+// page that is lost), rounded once: the product with the reciprocal and one
+// correction by the exact remainder (Markstein), three operations instead of
+// the ten of a division (for a power of two the first is exact already).
 struct PageScale {
-  float scale, ratio;
-  bool lost, grows;
+  float scale, inv, ratio;
+  bool grows;
   __device__ __forceinline__ float value(uint32_t bits16) const {
-    const float v = fminf(fmaxf(bf16_to_f32(bits16), -kLargest), kLargest);
-    return lost ? 0.0f : v / scale;
+    const float v = __builtin_amdgcn_fmed3f(bf16_to_f32(bits16), -kLargest, kLargest);
+    const float q = v * inv;
+    return fmaf(fmaf(-q, scale, v), inv, q);
   }
 };
 
@@ -364,12 +363,13 @@ __device__ __forceinline__ PageScale page_scale(AppendShared& sh, int tid, uint3
     for (int i = 0; i < kTeam; ++i) most = max(most, sh.largest[i]);
     __syncthreads();  // read before the next run writes
   }
+  const bool lost = most >= 0x7f80 || old != old;  // not finite, or the page was lost before
   PageScale p;
-  p.lost = most >= 0x7f80 || old != old;  // not finite, or the page was lost before
-  p.scale = p.lost ? __uint_as_float(0x7fc00000u) : fmaxf(old, scale_for<kFp8>((uint32_t)most));
-  p.grows = !p.lost && off > 0 && p.scale > old;
-  p.ratio = p.grows ? old / p.scale : 1.0f;
-  if (tid == 0 && (off == 0 || p.lost || p.grows)) *scale_at = p.scale;
+  p.scale = lost ? 0.0f : fmaxf(old, scale_for<kFp8>((uint32_t)most));
+  p.inv = lost ? 0.0f : 1.0f / p.scale;
+  p.grows = !lost && off > 0 && p.scale > old;
+  p.ratio = p.grows ? old * p.inv : 1.0f;
+  if (tid == 0 && (off == 0 || lost || p.grows)) *scale_at = lost ? __uint_as_float(0x7fc00000u) : p.scale;
   return p;
 }
 
@@ -530,22 +530,21 @@ __device__ __forceinline__ void append_values(const Append& a, AppendShared& sh,
 // 1)) of KV head h, keys (k = 0) or values; a long run by the block's four
 // waves, a short one by one of them.
 template <int D, bool kFp8>
-__global__ void __launch_bounds__(kAppendThreads) k_kv8_append(const Append a) {
+__global__ void __launch_bounds__(kAppendThreads, 6) k_kv8_append(const Append a) {
   __shared__ AppendShared sh;
   const int h = blockIdx.y, w = wave_id(), l = lane_id(), page = 1 << a.shift;
   const int most = a.pages << a.shift;  // (the host checks that it is an int)
   const int c0 = blockIdx.x * a.chunk;
-  // lane l: the slot of row c0 - 1 + l
-  const int mine = c0 - 1 + l;
-  const int slot = mine >= 0 && mine < a.rows ? a.slots[mine] : -1;
-  const int before = __shfl_up(slot, 1, kWave);
-  const bool valid = slot >= 0 && slot < most;
-  const bool begins = valid && l >= 1 && l <= a.chunk && !((slot & (page - 1)) != 0 && before == slot - 1);
+  // lane l: the slot of row c0 + l
+  const int slot = c0 + l < a.rows ? a.slots[c0 + l] : -1;
+  int before = __shfl_up(slot, 1, kWave);
+  if (l == 0) before = c0 > 0 ? a.slots[c0 - 1] : -1;
+  const bool begins = slot >= 0 && slot < most && l < a.chunk && !((slot & (page - 1)) != 0 && before == slot - 1);
   int turn = 0;
   for (uint64_t heads = __ballot(begins); heads; heads &= heads - 1) {
     const int at = __builtin_ctzll(heads), first = __builtin_amdgcn_readlane(slot, at);
     Run run;
-    run.r0 = c0 - 1 + at;
+    run.r0 = c0 + at;
     run.id = first >> a.shift;
     run.off = first & (page - 1);
     const uint64_t on = __ballot(l > at && slot == first + (l - at) && run.off + (l - at) < page);
@@ -1599,9 +1598,10 @@ extern "C" int lfm25_kv8_append(const lfm25_kv8_append_call* call, lfm25_stream_
   a.scales[0] = c.key_scales, a.scales[1] = c.value_scales;
   a.slots = c.slots;
   a.rows = c.rows, a.kv = c.kv_heads, a.pages = c.pages, a.shift = page_shift(c.page);
-  // few rows: a single token of a request for each wave; many: blocks for a
-  // quarter of a page of 64 or less, most of which find no run to begin
-  a.chunk = c.rows <= 512 ? 4 : 16;
+  // Few rows: a single token of a request for each wave. Many: a page's worth,
+  // since a block that finds no run to begin costs as much to start as any
+  // (4,096 rows in pages of 64: 19.7 us with 16 rows a block, 7.8 with 64).
+  a.chunk = c.rows <= 512 ? 4 : std::min(c.page, kWave);
   const dim3 grid((unsigned)((c.rows + (int64_t)a.chunk - 1) / a.chunk), (unsigned)c.kv_heads, 2), block(kAppendThreads);
   if (c.head_dim == 64) {
     if (c.format == LFM25_KV8_FP8) hipLaunchKernelGGL((k_kv8_append<64, true>), grid, block, 0, stream, a);
