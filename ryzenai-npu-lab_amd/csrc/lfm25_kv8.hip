@@ -607,11 +607,13 @@ struct Attend {
   const int* past;
   const int* starts;
   uint16_t* out;
-  float* part;      // [splits][rows][heads][D], each part's own result
-  float2* part_ml;  // [splits][rows][heads]: maximum, sum
+  float* part;      // results of parts: [narrow part][16 columns][D], [wide part][128 columns][D]
+  float2* part_ml;  // and their maxima and sums
   int* status;
   int width, rows, kv, group, pages, shift, requests, max_rows;
-  int narrow_splits, wide_splits, wide_blocks;
+  int narrow_splits, wide_splits, wide_blocks, early_blocks, narrow_blocks;
+  int narrow_items;     // of a block, beside wide tiles
+  size_t narrow_parts;  // columns of the narrow parts in `part`
   float scale;  // log2(e) * the softmax scale
 };
 
@@ -757,35 +759,49 @@ __device__ __forceinline__ float part_weight(float m, float all, float sum) {
 // ---- few columns: single tokens
 //
 // Up to 16 columns (rows x query heads of one KV head) of one request. Each
-// wave takes every fourth unit of the block's range and reads keys and values
-// from the cache straight into the operands' registers, the next unit's while
-// this one is computed: no LDS, no barrier until the waves' sums are joined.
-constexpr int kNarrowWaves = 4;
-
+// wave takes every kWaves-th unit of the block's range and reads keys and
+// values from the cache straight into the operands' registers, the next
+// unit's while this one is computed (and the page numbers of the one after):
+// no LDS, no barrier until the waves' sums are joined.
 template <int D>
 struct NarrowUnit {
   uint4 k[4][D / 64];
   uint4 v[D / 16];
-  Scales s;  // of this lane's segment, l / 16
+  float ks, vs;  // of this lane's segment, l / 16
   bool bad;
 };
+struct NarrowIds {
+  int k, v;  // this lane's pages, as the table has them
+};
+
+// The pages of unit u: keys' rows are positions 16 (r / 4) + 4 t + r % 4 of
+// operand row r = l % 16, values segment l / 16. Past the last position: 0.
+__device__ __forceinline__ NarrowIds narrow_ids(const Attend& a, const int* row, int len, int u) {
+  const int l = lane_id(), at_k = u * kUnit + 16 * ((l & 15) >> 2), at_v = u * kUnit + 16 * (l >> 4);
+  NarrowIds x{0, 0};
+  if (at_k < len) x.k = row[at_k >> a.shift];
+  if (at_v < len) x.v = row[at_v >> a.shift];
+  return x;
+}
 
 template <int D>
-__device__ __forceinline__ void narrow_load(const Attend& a, const int* row, int h, int len, int u, NarrowUnit<D>& x) {
+__device__ __forceinline__ void narrow_load(const Attend& a, int h, int u, const NarrowIds& id, NarrowUnit<D>& x) {
   const int l = lane_id(), r = l & 15, g = l >> 4, page = 1 << a.shift;
-  bool bad_k;
   const int at_k = u * kUnit + 16 * (r >> 2), at_v = u * kUnit + 16 * g;
-  const int id_k = page_at(a, row, at_k, len, bad_k), id_v = page_at(a, row, at_v, len, x.bad);
-  const uint8_t* k = a.k + ((((size_t)id_k * a.kv + h) << a.shift) + (at_k & (page - 1)) + (r & 3)) * D + g * (D / 4);
+  const uint32_t id_k = (uint32_t)id.k < (uint32_t)a.pages ? id.k : 0, id_v = (uint32_t)id.v < (uint32_t)a.pages ? id.v : 0;
+  x.bad = (uint32_t)id.v >= (uint32_t)a.pages;
+  const uint32_t page_bytes = (uint32_t)((a.kv << a.shift) * D), head_bytes = (uint32_t)((h << a.shift) * D);
+  const uint8_t* k = a.k + ((size_t)id_k * page_bytes + (head_bytes + (uint32_t)(((at_k & (page - 1)) + (r & 3)) * D + g * (D / 4))));
 #pragma unroll
   for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) x.k[t][c] = *reinterpret_cast<const uint4*>(k + (size_t)(4 * t) * D + 16 * c);
-  const size_t head = (size_t)id_v * a.kv + h;
-  const uint8_t* v = a.v + ((head * D + r) << a.shift) + (at_v & (page - 1));
+    for (int c = 0; c < D / 64; ++c) x.k[t][c] = *reinterpret_cast<const uint4*>(k + (4 * t) * D + 16 * c);
+  const uint8_t* v = a.v + ((size_t)id_v * page_bytes + (head_bytes + (uint32_t)((r << a.shift) + (at_v & (page - 1)))));
 #pragma unroll
-  for (int t = 0; t < D / 16; ++t) x.v[t] = *reinterpret_cast<const uint4*>(v + ((size_t)(16 * t) << a.shift));
-  x.s = Scales{a.ks[head], a.vs[head]};  // (as they are: turned into what they are used as when they are)
+  for (int t = 0; t < D / 16; ++t) x.v[t] = *reinterpret_cast<const uint4*>(v + ((16 * t) << a.shift));
+  const size_t head = (size_t)id_v * (uint32_t)a.kv + h;
+  x.ks = a.ks[head];
+  x.vs = a.vs[head];
 }
 
 template <int D, int kWaves>
@@ -794,15 +810,27 @@ struct NarrowShared {
   float o[kWaves][16][D + 4];
 };
 
-template <int D, bool kFp8, int kWaves>
-__device__ __forceinline__ void narrow_block(const Attend& a, int index, NarrowShared<D, kWaves>& sh) {
+// The part of a request's units that split sp takes.
+__device__ __forceinline__ int narrow_per(int units, int splits) { return (units + splits - 1) / splits; }
+
+// Item `index` (request, part, KV head) by kWaves waves, this one number w. A
+// block's items, if it has several, meet at its barrier.
+template <int D, bool kFp8, int kWaves, bool kAlone>
+__device__ __forceinline__ void narrow_block(const Attend& a, int index, int w, NarrowShared<D, kWaves>& sh) {
   const int h = index % a.kv, sp = index / a.kv % a.narrow_splits, b = index / a.kv / a.narrow_splits;
   Request rq;
-  if (!request_at(a, b, rq) || !rq.narrow) return;
-  const int units = (rq.len + kUnit - 1) / kUnit, per = (units + a.narrow_splits - 1) / a.narrow_splits;
+  if (kAlone) {
+    if (!request_at(a, b, rq) || !rq.narrow) return;
+  } else if (b >= a.requests || !request_at(a, b, rq) || !rq.narrow) {
+    rq.len = rq.count = 0;
+  }
+  const int units = (rq.len + kUnit - 1) / kUnit, per = narrow_per(units, a.narrow_splits);
   const int u0 = sp * per, u1 = min(units, u0 + per);
-  if (sp > 0 && u0 >= u1) return;  // (the combination knows which parts there are)
-  const int w = wave_id(), l = lane_id(), r = l & 15, g = l >> 4;
+  if (sp > 0 && u0 >= u1) {  // (the combination knows which parts there are)
+    if (kAlone) return;
+    rq.count = 0;
+  }
+  const int l = lane_id(), r = l & 15, g = l >> 4;
   const int* row = a.table + (size_t)b * a.width;
   const int columns = rq.count * a.group;
   // this lane's column: query row i, query head j of the KV head
@@ -811,9 +839,11 @@ __device__ __forceinline__ void narrow_block(const Attend& a, int index, NarrowS
   const int pos = live ? rq.past + ci : -1;
   NarrowUnit<D> next;
   int u = u0 + w;
-  if (u < u1) narrow_load<D>(a, row, h, rq.len, u, next);
+  NarrowIds ids = narrow_ids(a, row, rq.len, u);
+  if (u < u1) narrow_load<D>(a, h, u, ids, next);
+  ids = narrow_ids(a, row, rq.len, u + kWaves);
   bf16x8 q[D / 32];
-  {
+  if (kAlone || columns > 0) {
     const uint16_t* src = a.q + (size_t)(rq.row0 + (live ? ci : 0)) * a.q_stride + (size_t)(h * a.group + (live ? cj : 0)) * D + g * (D / 4);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
@@ -829,7 +859,8 @@ __device__ __forceinline__ void narrow_block(const Attend& a, int index, NarrowS
   for (int t = 0; t < D / 16; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   for (; u < u1; u += kWaves) {
     NarrowUnit<D> x = next;
-    if (u + kWaves < u1) narrow_load<D>(a, row, h, rq.len, u + kWaves, next);
+    if (u + kWaves < u1) narrow_load<D>(a, h, u + kWaves, ids, next);
+    ids = narrow_ids(a, row, rq.len, u + 2 * kWaves);
     f32x4 s[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -842,7 +873,7 @@ __device__ __forceinline__ void narrow_block(const Attend& a, int index, NarrowS
     }
     const int at = u * kUnit + 16 * g;  // this lane's first position
     const bool inside = at < rq.len;
-    Scales sc{x.s.ks * a.scale, scale_log2(x.s.lv)};
+    Scales sc{x.ks * a.scale, scale_log2(x.vs)};
     if (x.bad) raise(a.status, kStatusPage);
     const bool none = x.bad || !(sc.lv > -INFINITY);  // the segment's values count as 0
     if (x.bad || sc.lv != sc.lv) sc.ks = nan_of();
@@ -923,7 +954,7 @@ __device__ __forceinline__ void narrow_block(const Attend& a, int index, NarrowS
     *reinterpret_cast<f32x4*>(&sh.o[w][r][16 * t + 4 * g]) = o[t] * inv * unit;
   __syncthreads();
   const int heads = a.kv * a.group;
-  for (int e = threadIdx.x; e < columns * (D / 4); e += kWaves * kWave) {
+  for (int e = w * kWave + l; e < columns * (D / 4); e += kWaves * kWave) {
     const int c = e / (D / 4), d = 4 * (e % (D / 4));
     float all = -INFINITY;
 #pragma unroll
@@ -941,7 +972,7 @@ __device__ __forceinline__ void narrow_block(const Attend& a, int index, NarrowS
       if (rq.past + i >= 0) y = uint2{pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3])};
       *reinterpret_cast<uint2*>(a.out + at * D + d) = y;
     } else {
-      const size_t part = (size_t)sp * a.rows * heads + at;
+      const size_t part = (size_t)index * 16 + c;
       if (total == 0.0f) acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       *reinterpret_cast<f32x4*>(a.part + part * D + d) = acc;
       if (d == 0) a.part_ml[part] = float2{all, total};
@@ -949,10 +980,10 @@ __device__ __forceinline__ void narrow_block(const Attend& a, int index, NarrowS
   }
 }
 
-template <int D, bool kFp8>
-__global__ void __launch_bounds__(kNarrowWaves* kWave, D == 64 ? 4 : 2) k_kv8_attend_narrow(const Attend a) {
-  __shared__ NarrowShared<D, kNarrowWaves> sh;
-  narrow_block<D, kFp8, kNarrowWaves>(a, blockIdx.x, sh);
+template <int D, bool kFp8, int kWaves>
+__global__ void __launch_bounds__(kWaves* kWave, D == 64 ? 4 : 2) k_kv8_attend_narrow(const Attend a) {
+  extern __shared__ uint4 dynamic[];
+  narrow_block<D, kFp8, kWaves, true>(a, blockIdx.x, wave_id(), *reinterpret_cast<NarrowShared<D, kWaves>*>(dynamic));
 }
 
 // ---- many columns: prompt chunks
@@ -978,6 +1009,10 @@ struct Wide {
   static constexpr int kGroups = D == 64 ? 3 : 2, kWaves = kGroups * kWideWaves, kThreads = kWaves * kWave;
 };
 
+struct Found {
+  int request, tile;  // request -1: none
+  int waves[16], few[16];
+};
 template <int D>
 struct WideStages {
   uint4 k[2][kUnit * (D / 8)];  // [position][dim], rows of D / 8 16-byte slots
@@ -991,8 +1026,7 @@ struct WideShared {
     f32x4 o[Wide<D>::kGroups - 1][kWideColumns][D / 4 + 1];  // the groups' results, to be joined
   };
   float2 ml[Wide<D>::kGroups - 1][kWideColumns];
-  int found[2];
-  int waves[Wide<D>::kWaves];
+  Found found;
 };
 
 // 16 rows read at one slot number spread over all 64 banks (two 128-byte rows
@@ -1197,11 +1231,21 @@ __device__ __forceinline__ void wide_unit(const WideStages<D>& sh, int first, in
     }
 }
 
-// The request and tile of this block's item, among the wide requests' tiles
-// in order. found: request (-1: none), tile within it.
-template <int D>
-__device__ __forceinline__ void wide_find(const Attend& a, int item, WideShared<D>& sh) {
-  const int each = (a.requests + Wide<D>::kThreads - 1) / Wide<D>::kThreads, b0 = threadIdx.x * each;
+// The wide requests' tiles in order, each request's longest first, each in
+// `splits` parts of its keys. Where there is more than one request the host
+// cannot know how many tiles there are; the parts are then as many as fill
+// what the narrow requests leave of the chip, at most a.wide_splits.
+constexpr int kWideParts = 256, kLeastPart = 4;  // blocks that parts are made for; units in a part
+struct WideItem {
+  int b, tile, sp, splits, part;  // part: number of this part in the workspace
+};
+
+__device__ __forceinline__ int wide_per(int units, int splits) { return max((units + splits - 1) / splits, kLeastPart); }
+
+// Item `index` (head first) of the block, b < 0 if there is none.
+template <int kThreads>
+__device__ __forceinline__ WideItem wide_find(const Attend& a, int index, bool whole_tiles, Found& sh) {
+  const int each = (a.requests + kThreads - 1) / kThreads, b0 = threadIdx.x * each;
   const int l = lane_id(), w = wave_id();
   const auto tiles_of = [&](int b) {
     if (b >= a.requests) return 0;
@@ -1209,53 +1253,69 @@ __device__ __forceinline__ void wide_find(const Attend& a, int item, WideShared<
     if (s0 < 0 || s1 <= s0 || s1 > a.rows || s1 - s0 > a.max_rows || (int64_t)(s1 - s0) * a.group <= 16) return 0;
     return (int)(((int64_t)(s1 - s0) * a.group + kWideColumns - 1) / kWideColumns);
   };
-  int mine = 0;
-  for (int j = 0; j < each; ++j) mine += tiles_of(b0 + j);
-  int upto = mine;
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const int x = __shfl_up(upto, d, kWave);
-    if (l >= d) upto += x;
+  int mine = 0, few = 0;  // tiles, and requests that have none
+  for (int j = 0; j < each; ++j) {
+    const int n = tiles_of(b0 + j);
+    mine += n;
+    few += n == 0 && b0 + j < a.requests;
   }
-  if (l == kWave - 1) sh.waves[w] = upto;
-  if (threadIdx.x == 0) sh.found[0] = -1;
+  int upto = wave_sums(mine);
+  const int few_upto = wave_sums(few);
+  if (l == kWave - 1) sh.waves[w] = upto, sh.few[w] = few_upto;
+  if (threadIdx.x == 0) sh.request = -1;
   __syncthreads();
-  int total = 0;
-  for (int i = 0; i < Wide<D>::kWaves; ++i) {
+  int total = 0, others = 0;
+#pragma unroll
+  for (int i = 0; i < kThreads / kWave; ++i) {
     if (i == w) upto += total;
     total += sh.waves[i];
+    others += sh.few[i];
   }
+  WideItem x;
+  x.splits = a.wide_splits;
+  if (a.requests > 1) {
+    const int free = kWideParts - (int)min((int64_t)kWideParts, (int64_t)others * a.kv * a.narrow_splits / a.narrow_items);
+    x.splits = max(1, min(a.wide_splits, free / max(1, total * a.kv)));
+  }
+  const int h = index % a.kv, item = index / a.kv, rank = whole_tiles ? item : item / x.splits;
+  x.sp = whole_tiles ? 0 : item - rank * x.splits;
+  x.part = (rank * a.kv + h) * x.splits + x.sp;
   int first = upto - mine;
-  if (item >= first && item < upto) {
+  if (rank >= first && rank < upto) {
     for (int j = 0; j < each; ++j) {
       const int n = tiles_of(b0 + j);
-      if (item >= first && item < first + n) {
-        sh.found[0] = b0 + j;
-        sh.found[1] = n - 1 - (item - first);  // the longest first
+      if (rank >= first && rank < first + n) {
+        sh.request = b0 + j;
+        sh.tile = n - 1 - (rank - first);
       }
       first += n;
     }
   }
   __syncthreads();
+  x.b = __builtin_amdgcn_readfirstlane(sh.request);
+  x.tile = __builtin_amdgcn_readfirstlane(sh.tile);
+  return x;
+}
+
+// Positions that a tile of columns from c0 on sees, and its last query row.
+__device__ __forceinline__ int wide_end(const Attend& a, const Request& rq, int c0) {
+  const int last = (min(c0 + kWideColumns, rq.count * a.group) - 1) / a.group;
+  const int64_t end = (int64_t)rq.past + last + 1;
+  return end < 0 ? 0 : end > rq.cap ? rq.cap : (int)end;
 }
 
 template <int D, bool kFp8>
 __device__ __forceinline__ void wide_block(const Attend& a, int index, WideShared<D>& sh) {
-  const int h = index % a.kv, sp = index / a.kv % a.wide_splits;
-  const int w = wave_id(), l = lane_id();
-  wide_find<D>(a, index / a.kv / a.wide_splits, sh);
-  const int b = __builtin_amdgcn_readfirstlane(sh.found[0]);
-  if (b < 0) return;
+  const int h = index % a.kv, w = wave_id(), l = lane_id();
+  const WideItem item = wide_find<Wide<D>::kThreads>(a, index, false, sh.found);
+  if (item.b < 0) return;
   Request rq;
-  if (!request_at(a, b, rq)) return;
-  const int* row = a.table + (size_t)b * a.width;
-  const int columns = rq.count * a.group, c0 = __builtin_amdgcn_readfirstlane(sh.found[1]) * kWideColumns;
-  const int last = (min(c0 + kWideColumns, columns) - 1) / a.group;  // the tile's last query row
-  const int64_t end64 = (int64_t)rq.past + last + 1;
-  const int end = end64 < 0 ? 0 : end64 > rq.cap ? rq.cap : (int)end64;
-  const int units = (rq.len + kUnit - 1) / kUnit, per = (units + a.wide_splits - 1) / a.wide_splits;
-  const int u0 = sp * per, u1 = min((end + kUnit - 1) / kUnit, u0 + per);
-  if (sp > 0 && u0 >= u1) return;
+  if (!request_at(a, item.b, rq)) return;
+  const int* row = a.table + (size_t)item.b * a.width;
+  const int columns = rq.count * a.group, c0 = item.tile * kWideColumns, end = wide_end(a, rq, c0);
+  const int units = (rq.len + kUnit - 1) / kUnit, per = wide_per(units, item.splits);
+  const int u0 = item.sp * per, u1 = min((end + kUnit - 1) / kUnit, u0 + per);
+  if (item.sp > 0 && u0 >= u1) return;
   constexpr int kGroups = Wide<D>::kGroups;
   const int group = w / kWideWaves, w4 = w % kWideWaves;
   WideStages<D>& mine = sh.group[group];
@@ -1365,12 +1425,12 @@ __device__ __forceinline__ void wide_block(const Attend& a, int index, WideShare
   float share[kGroups], total = share[0] = part_weight(x.m, all, x.sum);
 #pragma unroll
   for (int g = 1; g < kGroups; ++g) total += share[g] = part_weight(sh.ml[g - 1][c].x, all, sh.ml[g - 1][c].y);
-  const bool single = a.wide_splits == 1, none = !single && total == 0.0f;
+  const bool single = item.splits == 1, none = !single && total == 0.0f;
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) share[g] = none ? 0.0f : share[g] / total;
   const int heads = a.kv * a.group;
   const size_t at = (size_t)(rq.row0 + ci) * heads + h * a.group + cj;
-  const size_t part = (size_t)sp * a.rows * heads + at;
+  const size_t part = a.narrow_parts + (size_t)item.part * kWideColumns + c;  // (narrow parts come first)
 #pragma unroll
   for (int t = 0; t < D / 32; ++t)
 #pragma unroll
@@ -1396,79 +1456,110 @@ __device__ __forceinline__ void wide_block(const Attend& a, int index, WideShare
 template <int D>
 union BothShared {
   WideShared<D> wide;
-  NarrowShared<D, Wide<D>::kWaves> narrow;
+  NarrowShared<D, 4> narrow[Wide<D>::kWaves / 4];
 };
 
 template <int D, bool kFp8>
 __global__ void __launch_bounds__(Wide<D>::kThreads, Wide<D>::kWaves / 4) k_kv8_attend_both(const Attend a) {
   extern __shared__ uint4 dynamic[];
   BothShared<D>& sh = *reinterpret_cast<BothShared<D>*>(dynamic);
-  if ((int)blockIdx.x < a.wide_blocks) wide_block<D, kFp8>(a, blockIdx.x, sh.wide);
-  else narrow_block<D, kFp8, Wide<D>::kWaves>(a, blockIdx.x - a.wide_blocks, sh.narrow);
+  // wide tiles first, since they take longest; those past the first round of
+  // the chip, which may be none, behind the narrow requests
+  int i = blockIdx.x;
+  if (i >= a.early_blocks) i = i < a.early_blocks + a.narrow_blocks ? i + (a.wide_blocks - a.early_blocks) : i - a.narrow_blocks;
+  if (i < a.wide_blocks) {
+    wide_block<D, kFp8>(a, i, sh.wide);
+  } else {
+    const int w = wave_id();
+    narrow_block<D, kFp8, 4, false>(a, (i - a.wide_blocks) * (Wide<D>::kWaves / 4) + w / 4, w % 4, sh.narrow[w / 4]);
+  }
 }
 
-// ---- the parts of a split range of keys joined, in the parts' order: a wave
-// for one row and query head.
-constexpr int kCombineWaves = 4;
+// ---- the parts of a split range of keys joined, in the parts' order
+//
+// Four blocks for a request and KV head's narrow columns, or for one wide tile.
+constexpr int kCombineThreads = 256, kQuarters = 4, kMostShares = 512;  // parts x columns: 64 x 4, 16 x 32
 
-// The request that row x belongs to (requests if it is behind the last), by
-// one wave: 64 of the offsets at a time.
-__device__ __forceinline__ int request_of_row(const int* starts, int n, int x) {
-  const int l = lane_id(), step = (n + kWave) / kWave;  // step * 64 > n
-  const int at = l * step;
-  const int coarse = __popcll(__ballot(at <= n && starts[min(at, n)] <= x)) - 1;
-  if (coarse < 0) return n;
-  int found = coarse * step;
-  for (int i0 = 1; i0 < step; i0 += kWave) {
-    const int i = coarse * step + i0 + l;
-    found += __popcll(__ballot(i0 + l < step && i <= n && starts[min(i, n)] <= x));
+struct CombineShared {
+  Found found;
+  float share[kMostShares];
+};
+
+// Sum or maximum over a lane's group of 16 or of all 64.
+template <bool kAll>
+__device__ __forceinline__ float lanes_max(float v) { return kAll ? wave_max(v) : row16_max(v); }
+template <bool kAll>
+__device__ __forceinline__ float lanes_sum(float v) { return kAll ? wave_sum(v) : row16_sum(v); }
+
+// Each part's share of its column, a lane for each part.
+template <bool kAll>
+__device__ __forceinline__ void combine_shares(const float2* ml, size_t stride, int parts, int columns, float* share) {
+  constexpr int kLanes = kAll ? kWave : 16;
+  const int p = threadIdx.x % kLanes;
+  for (int c = threadIdx.x / kLanes; c < columns; c += kCombineThreads / kLanes) {
+    float2 x{-INFINITY, 0.0f};
+    if (p < parts) x = ml[p * stride + c];
+    const float s = part_weight(x.x, lanes_max<kAll>(x.x), x.y);
+    const float of = s / lanes_sum<kAll>(s);
+    if (p < parts) share[p * columns + c] = of;
   }
-  return found;
 }
 
 template <int D>
-__global__ void __launch_bounds__(kCombineWaves* kWave) k_kv8_combine(const Attend a) {
-  const int heads = a.kv * a.group, l = lane_id();
-  const int64_t item = (int64_t)blockIdx.x * kCombineWaves + wave_id();
-  if (item >= (int64_t)a.rows * heads) return;
-  const int most = max(a.narrow_splits, a.wide_splits);
-  const size_t stride = (size_t)a.rows * heads;
-  // asked for before it is known how many parts there are
-  float2 ml{-INFINITY, 0.0f};
-  if (l < most) ml = a.part_ml[l * stride + item];
-  const int x = (int)(item / heads);
-  const int b = __builtin_amdgcn_readfirstlane(request_of_row(a.starts, a.requests, x));
-  if (b >= a.requests) return;
+__global__ void __launch_bounds__(kCombineThreads) k_kv8_combine(const Attend a, int wide_items) {
+  __shared__ CombineShared sh;
+  const int quarter = blockIdx.x % kQuarters, item_at = blockIdx.x / kQuarters;
+  const bool wide = item_at < wide_items;
+  const int index = wide ? item_at : item_at - wide_items, h = index % a.kv;
   Request rq;
-  if (!request_at(a, b, rq)) return;
-  const int splits = rq.narrow ? a.narrow_splits : a.wide_splits;
-  if (splits == 1) return;
-  const int64_t pos = (int64_t)rq.past + (x - rq.row0);
-  const int units = (rq.len + kUnit - 1) / kUnit, per = (units + splits - 1) / splits;
-  const int seen = (int)((min(pos + 1, (int64_t)rq.len) + kUnit - 1) / kUnit);  // units that the row sees
-  const int parts = pos < 0 ? 0 : (seen + per - 1) / per;                      // 1 .. splits, at most 64
-  if (l >= parts) ml = float2{-INFINITY, 0.0f};
-  const float all = wave_max(ml.x);
-  float share = part_weight(ml.x, all, ml.y);
-  share /= wave_sum(share);
-  float acc[D / 64] = {};
-  const float* from = a.part + item * D + l;
-  constexpr int kAhead = 8;
-  for (int i0 = 0; i0 < parts; i0 += kAhead) {
-    float y[kAhead][D / 64];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) y[i][c] = from[min(i0 + i, parts - 1) * stride * D + 64 * c];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const float f = i0 + i < parts ? lane_value(share, min(i0 + i, kWave - 1)) : 0.0f;
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) acc[c] += i0 + i < parts ? f * y[i][c] : 0.0f;
-    }
+  int parts, columns, c0 = 0, stride;  // columns of the item, the first of this block's
+  size_t from;  // column 0 of part 0
+  if (wide) {
+    const WideItem item = wide_find<kCombineThreads>(a, index, true, sh.found);
+    if (item.b < 0 || item.splits == 1 || !request_at(a, item.b, rq)) return;
+    c0 = item.tile * kWideColumns;
+    columns = min(kWideColumns, rq.count * a.group - c0);
+    const int units = (rq.len + kUnit - 1) / kUnit, per = wide_per(units, item.splits);
+    parts = ((wide_end(a, rq, c0) + kUnit - 1) / kUnit + per - 1) / per;
+    from = a.narrow_parts + (size_t)item.part * kWideColumns;
+    stride = kWideColumns;
+  } else {
+    const int b = index / a.kv;
+    if (a.narrow_splits == 1 || !request_at(a, b, rq) || !rq.narrow) return;
+    columns = rq.count * a.group;
+    const int units = (rq.len + kUnit - 1) / kUnit;
+    parts = units > 0 ? (units + narrow_per(units, a.narrow_splits) - 1) / narrow_per(units, a.narrow_splits) : 0;
+    from = ((size_t)b * a.narrow_splits * a.kv + h) * 16;
+    stride = 16 * a.kv;
   }
+  parts = max(parts, 1);  // (the first is there in any case)
+  const int mine = wide ? kWideColumns / kQuarters : 16 / kQuarters;
+  from += quarter * mine;
+  columns = min(columns - quarter * mine, mine);
+  c0 += quarter * mine;
+  if (columns <= 0) return;
+  if (parts <= 16) combine_shares<false>(a.part_ml + from, stride, parts, columns, sh.share);
+  else combine_shares<true>(a.part_ml + from, stride, parts, columns, sh.share);
+  __syncthreads();
+  const int heads = a.kv * a.group;
+  for (int e = threadIdx.x; e < columns * (D / 4); e += kCombineThreads) {
+    const int c = e / (D / 4), d = 4 * (e % (D / 4));
+    const float* const x = a.part + (from + c) * D + d;
+    f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int kAhead = 8;
+    for (int p0 = 0; p0 < parts; p0 += kAhead) {
+      f32x4 y[kAhead];
 #pragma unroll
-  for (int c = 0; c < D / 64; ++c) a.out[item * D + 64 * c + l] = pos < 0 ? (uint16_t)0 : f32_to_bf16(acc[c]);
+      for (int p = 0; p < kAhead; ++p) y[p] = *reinterpret_cast<const f32x4*>(x + (size_t)min(p0 + p, parts - 1) * stride * D);
+#pragma unroll
+      for (int p = 0; p < kAhead; ++p)
+        if (p0 + p < parts) acc += sh.share[(p0 + p) * columns + c] * y[p];
+    }
+    const int i = (c0 + c) / a.group, j = c0 + c - i * a.group;
+    uint2 y{0, 0};
+    if (rq.past + i >= 0) y = uint2{pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3])};
+    *reinterpret_cast<uint2*>(a.out + ((size_t)(rq.row0 + i) * heads + h * a.group + j) * D + d) = y;
+  }
 }
 
 // ------------------------------------------------------------------ host
@@ -1493,37 +1584,53 @@ bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0
 
 struct Splits {
   int narrow, wide;     // parts of a request's keys for each kind of request
+  int waves;            // of a narrow block, where there are no wide requests
   int64_t wide_tiles;   // most tiles that the rows can make
+  int64_t wide_blocks;  // and blocks for them
   bool has_wide;
 };
+constexpr int kMostWideParts = 16;
 
-// Parts of a request's keys, from what the host knows (the lengths are on the
-// device; the table's width bounds them): enough blocks to fill the chip (256
-// CUs, four narrow blocks or two wide ones each) where the requests alone do
-// not, of at least 256 positions (a unit for each of a narrow block's waves)
-// or 512. Beside wide tiles that fill the chip already the narrow requests
-// are divided only to keep one block's share to 8,192 positions.
-Splits splits_for(int32_t rows, int32_t requests, int32_t kv, int32_t group, int32_t max_rows, int32_t width, int32_t page) {
-  Splits s{1, 1, 0, false};
-  const int64_t positions = std::min<int64_t>((int64_t)width * page, INT32_MAX);
+// Waves of a block and parts of a request's keys, from what the host knows
+// (the lengths are on the device; the table's width bounds them).
+Splits splits_for(int32_t rows, int32_t requests, int32_t kv, int32_t group, int32_t max_rows, int32_t width, int32_t page,
+                  int32_t dim) {
+  Splits s{1, 1, 4, 0, 0, false};
+  const int64_t positions = std::min<int64_t>((int64_t)width * page, INT32_MAX), units = (positions + kUnit - 1) / kUnit;
   const auto parts = [&](int64_t wanted, int64_t blocks, int64_t least) {
     return (int)std::max<int64_t>(1, std::min({wanted / blocks, positions / least, (int64_t)kWave}));
   };
-  s.narrow = parts(1024, (int64_t)std::min(requests, rows) * kv, 256);
+  const int64_t blocks = (int64_t)std::min(requests, rows) * kv;
+  // a chip holds 4,096 waves of dim 64, 2,048 of dim 128
+  constexpr int most = 8;
+  const int64_t full = dim == 64 ? 4096 : 2048;
+  while (s.waves < most && units >= 2 * s.waves && blocks * s.waves < full) s.waves *= 2;
+  s.narrow = parts(full / s.waves, blocks, 128 * s.waves);
   s.has_wide = (int64_t)max_rows * group > 16;
   if (s.has_wide) {
+    s.waves = 4;  // beside wide tiles
     const int64_t columns = (int64_t)rows * group;
     s.wide_tiles = columns / kWideColumns + std::min<int64_t>(requests, columns / 17 + 1);
-    s.wide = parts(512, s.wide_tiles * kv, 512);
-    if (s.wide_tiles * kv >= 256) s.narrow = (int)std::min<int64_t>(s.narrow, (positions + 8191) / 8192);
+    if (requests == 1) {
+      s.wide_tiles = (columns + kWideColumns - 1) / kWideColumns;
+      s.wide = (int)std::min<int64_t>(parts(kWideParts, s.wide_tiles * kv, kLeastPart * kUnit), kMostWideParts);
+      s.wide_blocks = s.wide_tiles * kv * s.wide;
+    } else {
+      s.wide = (int)std::max<int64_t>(1, std::min<int64_t>(units / kLeastPart, kMostWideParts));
+      s.wide_blocks = s.wide > 1 ? std::max<int64_t>(s.wide_tiles * kv, kWideParts) : s.wide_tiles * kv;
+    }
+    // The narrow requests beside them are divided only to keep one block's
+    // share to 8,192 positions.
+    s.narrow = (int)std::min<int64_t>({s.narrow, (positions + 8191) / 8192, kWave});
   }
   return s;
 }
 
-size_t part_floats(const Splits& s, int64_t rows, int64_t heads, int64_t dim) {
-  const int most = std::max(s.narrow, s.wide);
-  return most == 1 ? 0 : (size_t)(most * rows * heads * (dim + 2));
+// Columns of the narrow and of the wide parts in the workspace.
+size_t narrow_columns(const Splits& s, int64_t requests, int64_t kv) {
+  return s.narrow > 1 ? (size_t)(requests * kv * s.narrow * 16) : 0;
 }
+size_t wide_columns(const Splits& s) { return s.has_wide && s.wide > 1 ? (size_t)kWideParts * kWideColumns : 0; }
 
 template <int kThreads, int kEach>
 void plan(const lfm25_kv8_plan_call& c, int shift, hipStream_t stream) {
@@ -1532,18 +1639,28 @@ void plan(const lfm25_kv8_plan_call& c, int shift, hipStream_t stream) {
                      c.next_cursor, c.status, shift);
 }
 
+template <int D, bool kFp8, int kWaves>
+void attend_narrow(const Attend& a, int64_t blocks, hipStream_t stream) {
+  hipLaunchKernelGGL((k_kv8_attend_narrow<D, kFp8, kWaves>), dim3((unsigned)blocks), dim3(kWaves * kWave),
+                     sizeof(NarrowShared<D, kWaves>), stream, a);
+}
+
 template <int D, bool kFp8>
 int attend(const Attend& a, const Splits& s, hipStream_t stream) {
   const int64_t narrow = (int64_t)a.requests * a.kv * a.narrow_splits;
-  if (s.has_wide)
-    hipLaunchKernelGGL((k_kv8_attend_both<D, kFp8>), dim3((unsigned)(a.wide_blocks + narrow)), dim3(Wide<D>::kThreads),
+  if (s.has_wide) {
+    hipLaunchKernelGGL((k_kv8_attend_both<D, kFp8>), dim3((unsigned)(a.wide_blocks + a.narrow_blocks)), dim3(Wide<D>::kThreads),
                        sizeof(BothShared<D>), stream, a);
-  else
-    hipLaunchKernelGGL((k_kv8_attend_narrow<D, kFp8>), dim3((unsigned)narrow), dim3(kNarrowWaves * kWave), 0, stream, a);
-  if (a.narrow_splits > 1 || a.wide_splits > 1) {
-    const int64_t items = (int64_t)a.rows * a.kv * a.group;
-    hipLaunchKernelGGL((k_kv8_combine<D>), dim3((unsigned)((items + kCombineWaves - 1) / kCombineWaves)),
-                       dim3(kCombineWaves * kWave), 0, stream, a);
+  } else if (s.waves == 4) {
+    attend_narrow<D, kFp8, 4>(a, narrow, stream);
+  } else {
+    attend_narrow<D, kFp8, 8>(a, narrow, stream);
+  }
+  if (s.narrow > 1 || (s.has_wide && s.wide > 1)) {
+    // (a tile in parts is one of at most kWideParts / 2)
+    const int wide_items = s.has_wide && s.wide > 1 ? kWideParts / 2 : 0;
+    const int64_t narrow_items = s.narrow > 1 ? (int64_t)a.requests * a.kv : 0;
+    hipLaunchKernelGGL((k_kv8_combine<D>), dim3((unsigned)((wide_items + narrow_items) * kQuarters)), dim3(kCombineThreads), 0, stream, a, wide_items);
   }
   return check_launch("lfm25_kv8_attention");
 }
@@ -1628,8 +1745,8 @@ extern "C" size_t lfm25_kv8_attention_workspace_bytes(int32_t rows, int32_t head
   if (page_shift(page) < 0 || (head_dim != 64 && head_dim != 128) ||
       !attend_shape(rows, heads, kv_heads, requests, max_rows, width, page))
     return 0;
-  const Splits s = splits_for(rows, requests, kv_heads, heads / kv_heads, std::min(max_rows, rows), width, page);
-  return 4 * part_floats(s, rows, heads, head_dim);
+  const Splits s = splits_for(rows, requests, kv_heads, heads / kv_heads, std::min(max_rows, rows), width, page, head_dim);
+  return 4 * (narrow_columns(s, requests, kv_heads) + wide_columns(s)) * (head_dim + 2);
 }
 
 extern "C" int lfm25_kv8_attention(const lfm25_kv8_attention_call* call, lfm25_stream_t stream) {
@@ -1650,9 +1767,9 @@ extern "C" int lfm25_kv8_attention(const lfm25_kv8_attention_call* call, lfm25_s
   LFM25_REQUIRE(std::isfinite(c.scale) && c.scale >= 0.0f, "lfm25_kv8_attention: scale must be finite and not negative");
   LFM25_REQUIRE(c.reserved == 0, "lfm25_kv8_attention: reserved must be 0");
   const int group = c.heads / c.kv_heads, max_rows = std::min(c.max_rows, c.rows);
-  const Splits s = splits_for(c.rows, c.requests, c.kv_heads, group, max_rows, c.width, c.page);
-  const size_t floats = part_floats(s, c.rows, c.heads, c.head_dim);
-  LFM25_REQUIRE(floats == 0 || (c.workspace != nullptr && aligned16(c.workspace)),
+  const Splits s = splits_for(c.rows, c.requests, c.kv_heads, group, max_rows, c.width, c.page, c.head_dim);
+  const size_t columns = narrow_columns(s, c.requests, c.kv_heads) + wide_columns(s);
+  LFM25_REQUIRE(columns == 0 || (c.workspace != nullptr && aligned16(c.workspace)),
                 "lfm25_kv8_attention: needs a 16-byte aligned workspace of lfm25_kv8_attention_workspace_bytes()");
   Attend a{};
   a.q = c.query, a.q_stride = c.query_stride;
@@ -1661,12 +1778,16 @@ extern "C" int lfm25_kv8_attention(const lfm25_kv8_attention_call* call, lfm25_s
   a.table = c.block_table, a.past = c.past, a.starts = c.row_starts;
   a.out = c.output;
   a.part = static_cast<float*>(c.workspace);
-  a.part_ml = reinterpret_cast<float2*>(a.part + (size_t)std::max(s.narrow, s.wide) * c.rows * c.heads * c.head_dim);
+  a.part_ml = reinterpret_cast<float2*>(a.part + columns * c.head_dim);
+  a.narrow_parts = narrow_columns(s, c.requests, c.kv_heads);
   a.status = c.status;
   a.width = c.width, a.rows = c.rows, a.kv = c.kv_heads, a.group = group, a.pages = c.pages, a.shift = page_shift(c.page);
   a.requests = c.requests, a.max_rows = max_rows;
   a.narrow_splits = s.narrow, a.wide_splits = s.wide;
-  a.wide_blocks = (int)(s.wide_tiles * c.kv_heads * s.wide);
+  a.wide_blocks = (int)s.wide_blocks;
+  a.early_blocks = std::min(a.wide_blocks, kWideParts);
+  a.narrow_items = (c.head_dim == 64 ? Wide<64>::kWaves : Wide<128>::kWaves) / 4;
+  a.narrow_blocks = (int)(((int64_t)c.requests * c.kv_heads * s.narrow + a.narrow_items - 1) / a.narrow_items);
   a.scale = c.scale * 1.4426950408889634f;
   if (c.head_dim == 64) return c.format == LFM25_KV8_FP8 ? attend<64, true>(a, s, stream) : attend<64, false>(a, s, stream);
   return c.format == LFM25_KV8_FP8 ? attend<128, true>(a, s, stream) : attend<128, false>(a, s, stream);
