@@ -96,11 +96,12 @@ def test_attention_refuses(lab, change, message):
 
 def test_workspace_sizes(lab):
     size = lab.load_library().lfm25_kv8_attention_workspace_bytes
+    column = 4 * (64 + 2)
     assert size(4, 16, 8, 64, 4, 1, 3, 64) == 0            # too few positions to divide
     assert size(64, 16, 8, 64, 0, 1, 64, 64) == 0          # a refused call
-    parts = size(4, 16, 8, 64, 4, 1, 64, 64) / (4 * 16 * (64 + 2) * 4)
-    assert parts == 16                                     # 4,096 positions in parts of 256
-    assert size(1, 16, 8, 64, 1, 1, 1 << 20, 64) == 64 * 16 * 66 * 4  # 64 parts at most
+    assert size(4, 16, 8, 64, 4, 1, 64, 64) == 4 * 8 * 4 * 16 * column            # four parts of 1,024 positions
+    assert size(1, 16, 8, 64, 1, 1, 1 << 20, 64) == 8 * 64 * 16 * column          # 64 parts at most
+    assert size(512, 16, 8, 64, 2, 256, 64, 64) == 256 * 128 * column             # parts of tiles of 128 columns
 
 
 def test_ops_refuse_before_any_launch(lab):
