@@ -611,7 +611,9 @@ struct Attend {
   float2* part_ml;  // and their maxima and sums
   int* status;
   int width, rows, kv, group, pages, shift, requests, max_rows;
-  int narrow_splits, wide_splits, wide_blocks, early_blocks, narrow_blocks;
+  int narrow_share;  // parts that the narrow requests together are divided into, beside one each; 0: not divided
+  int narrow_least;  // least units of a part
+  int wide_splits, wide_blocks, early_blocks, narrow_blocks;
   int narrow_items;     // of a block, beside wide tiles
   size_t narrow_parts;  // columns of the narrow parts in `part`
   float scale;  // log2(e) * the softmax scale
@@ -634,7 +636,7 @@ __device__ __forceinline__ bool request_at(const Attend& a, int b, Request& r) {
   r.past = a.past[b];
   if (s1 == s0) return false;
   if (s0 < 0 || s1 < s0 || s1 > a.rows || s1 - s0 > a.max_rows) {
-    if (threadIdx.x == 0) raise(a.status, kStatusRows);
+    raise(a.status, kStatusRows);
     return false;
   }
   r.row0 = s0;
@@ -644,7 +646,7 @@ __device__ __forceinline__ bool request_at(const Attend& a, int b, Request& r) {
   r.past = min(r.past, INT32_MAX - r.count);  // (past any table either way; positions stay ints)
   r.len = len < 0 ? 0 : len > r.cap ? r.cap : (int)len;
   r.narrow = (int64_t)r.count * a.group <= 16;
-  if (len > r.cap && threadIdx.x == 0) raise(a.status, kStatusPage);
+  if (len > r.cap) raise(a.status, kStatusPage);
   return true;
 }
 
@@ -750,10 +752,17 @@ __device__ __forceinline__ float dot2(uint32_t p, uint32_t w, float sum) {
 // ratios as they are.
 constexpr float kSlack = 8.0f;
 
+constexpr int kMostNarrowParts = 64;  // of one request
+
 // A part's share of a whole: its sum against the common maximum, 0 for a part
 // that saw nothing (m = -inf).
 __device__ __forceinline__ float part_weight(float m, float all, float sum) {
   return (m == -INFINITY ? 0.0f : exp2_of(m - all)) * sum;
+}
+
+__device__ __forceinline__ int uniform_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ float uniform_of(float v, int lane) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
 }
 
 // ---- few columns: single tokens
@@ -810,26 +819,129 @@ struct NarrowShared {
   float o[kWaves][16][D + 4];
 };
 
-// The part of a request's units that split sp takes.
-__device__ __forceinline__ int narrow_per(int units, int splits) { return (units + splits - 1) / splits; }
+// The narrow requests' division into parts of `per` units, found by each wave
+// from the lengths: as many parts as fill the chip, whoever's keys they are,
+// since lengths in a batch differ as they like (a request of 100,000
+// positions beside one of 2,000: 44 us with the same number of parts for
+// each, 35 with parts of the same length).
+constexpr int kDivided = 256;  // requests, at most four a lane
+struct NarrowPart {
+  int b, sp;    // request and which of its parts
+  int first;    // its first part among all
+  int parts;    // how many it has
+  int per;
+};
 
-// Item `index` (request, part, KV head) by kWaves waves, this one number w. A
-// block's items, if it has several, meet at its barrier.
-template <int D, bool kFp8, int kWaves, bool kAlone>
+__device__ __forceinline__ uint32_t narrow_units(const Attend& a, int b, Request& rq) {
+  if (b >= a.requests || !request_at(a, b, rq) || !rq.narrow) return 0;
+  return max(1u, (uint32_t)(rq.len + kUnit - 1) / kUnit);
+}
+
+// Part number `at` (kPart) or the first part of request `at`, and the request;
+// false if there is none.
+template <bool kPart>
+__device__ __forceinline__ bool narrow_find(const Attend& a, int at, NarrowPart& x, Request& rq) {
+  constexpr int kEach = kDivided / kWave;
+  // Parts a little longer until there are no more than wanted (each request's
+  // last is shorter); with any length from the first on there are at most
+  // a.requests more.
+  constexpr int kTurns = 6;
+  const int l = lane_id();
+  const auto per_of = [&](uint32_t total, uint32_t most) {
+    total = (uint32_t)uniform_of(wave_sums((int)total), kWave - 1);
+    // (rounded to FP32: a bound for the combination's parts, 63 or 64)
+    const uint32_t bound = (uint32_t)__builtin_amdgcn_readfirstlane((int)wave_max((float)most)) / (kMostNarrowParts - 1) + 1;
+    return max(max((uint32_t)a.narrow_least, (total + a.narrow_share - 1) / a.narrow_share), bound);
+  };
+  if (a.requests <= kWave) {  // a lane each: no second look at the lengths
+    Request my;
+    const uint32_t units = narrow_units(a, l, my);
+    uint32_t per = per_of(units, units), mine;
+    int upto;
+    for (int turn = 0;; ++turn) {
+      mine = (units + per - 1) / per;
+      upto = wave_sums((int)mine);
+      if (turn == kTurns || uniform_of(upto, kWave - 1) <= a.narrow_share) break;
+      per += per / 16 + 1;
+    }
+    x.per = (int)per;
+    if (kPart) {
+      const uint64_t reach = __ballot(upto > at);
+      if (reach == 0) return false;
+      x.b = __builtin_ctzll(reach);
+    } else {
+      x.b = at;
+    }
+    x.first = uniform_of(upto - (int)mine, x.b);
+    x.parts = uniform_of((int)mine, x.b);
+    x.sp = kPart ? at - x.first : 0;
+    rq.row0 = uniform_of(my.row0, x.b), rq.count = uniform_of(my.count, x.b), rq.past = uniform_of(my.past, x.b);
+    rq.len = uniform_of(my.len, x.b), rq.cap = clamp_int((int64_t)a.width << a.shift);
+    return x.parts > 0;
+  }
+  const int each = (a.requests + kWave - 1) / kWave, b0 = l * each;
+  uint32_t units[kEach], total = 0, most = 0;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    Request my;
+    units[j] = j < each ? narrow_units(a, b0 + j, my) : 0;
+    total += units[j];
+    most = max(most, units[j]);
+  }
+  uint32_t per = per_of(total, most), parts[kEach];
+  int mine, upto;
+  for (int turn = 0;; ++turn) {
+    mine = 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      parts[j] = j < each ? (units[j] + per - 1) / per : 0;
+      mine += (int)parts[j];
+    }
+    upto = wave_sums(mine);
+    if (turn == kTurns || uniform_of(upto, kWave - 1) <= a.narrow_share) break;
+    per += per / 16 + 1;
+  }
+  int lane = at / each;
+  if (kPart) {
+    const uint64_t reach = __ballot(upto > at);
+    if (reach == 0) return false;
+    lane = __builtin_ctzll(reach);
+  }
+  x.per = (int)per;
+  x.b = lane * each;
+  x.first = uniform_of(upto - mine, lane);
+  x.parts = uniform_of((int)parts[0], lane);
+#pragma unroll
+  for (int j = 1; j < kEach; ++j)
+    if (j < each && (kPart ? at >= x.first + x.parts : x.b < at)) {
+      ++x.b;
+      x.first += x.parts;
+      x.parts = uniform_of((int)parts[j], lane);
+    }
+  x.sp = kPart ? at - x.first : 0;
+  return x.parts > 0 && request_at(a, x.b, rq);
+}
+
+// Item `index` (part, KV head) by kWaves waves, this one number w. A block's
+// items, if it has several, meet at its barrier.
+template <int D, bool kFp8, int kWaves, bool kAlone, bool kParts>
 __device__ __forceinline__ void narrow_block(const Attend& a, int index, int w, NarrowShared<D, kWaves>& sh) {
-  const int h = index % a.kv, sp = index / a.kv % a.narrow_splits, b = index / a.kv / a.narrow_splits;
+  const int h = index % a.kv;
+  NarrowPart part{index / a.kv, 0, 0, 1, INT32_MAX / 2};
   Request rq;
-  if (kAlone) {
-    if (!request_at(a, b, rq) || !rq.narrow) return;
-  } else if (b >= a.requests || !request_at(a, b, rq) || !rq.narrow) {
-    rq.len = rq.count = 0;
-  }
-  const int units = (rq.len + kUnit - 1) / kUnit, per = narrow_per(units, a.narrow_splits);
-  const int u0 = sp * per, u1 = min(units, u0 + per);
-  if (sp > 0 && u0 >= u1) {  // (the combination knows which parts there are)
+  bool some;
+  if (kParts && a.narrow_share > 0) some = narrow_find<true>(a, part.b, part, rq);
+  else some = part.b < a.requests && request_at(a, part.b, rq) && rq.narrow;
+  if (!some) {
     if (kAlone) return;
-    rq.count = 0;
+    rq.len = rq.count = 0;
+    part.b = 0;
   }
+  const int b = __builtin_amdgcn_readfirstlane(part.b);
+  rq.row0 = __builtin_amdgcn_readfirstlane(rq.row0), rq.count = __builtin_amdgcn_readfirstlane(rq.count);
+  rq.past = __builtin_amdgcn_readfirstlane(rq.past), rq.len = __builtin_amdgcn_readfirstlane(rq.len);
+  const int units = (rq.len + kUnit - 1) / kUnit;
+  const int u0 = part.sp * part.per, u1 = min(units, u0 + part.per);
   const int l = lane_id(), r = l & 15, g = l >> 4;
   const int* row = a.table + (size_t)b * a.width;
   const int columns = rq.count * a.group;
@@ -967,23 +1079,23 @@ __device__ __forceinline__ void narrow_block(const Attend& a, int index, int w, 
     for (int i = 0; i < kWaves; ++i) acc += (share[i] / total) * *reinterpret_cast<const f32x4*>(&sh.o[i][c][d]);
     const int i = c / a.group, j = c - i * a.group;
     const size_t at = (size_t)(rq.row0 + i) * heads + h * a.group + j;
-    if (a.narrow_splits == 1) {
+    if (part.parts == 1) {
       uint2 y{0, 0};
       if (rq.past + i >= 0) y = uint2{pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3])};
       *reinterpret_cast<uint2*>(a.out + at * D + d) = y;
     } else {
-      const size_t part = (size_t)index * 16 + c;
+      const size_t to = (size_t)index * 16 + c;
       if (total == 0.0f) acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      *reinterpret_cast<f32x4*>(a.part + part * D + d) = acc;
-      if (d == 0) a.part_ml[part] = float2{all, total};
+      *reinterpret_cast<f32x4*>(a.part + to * D + d) = acc;
+      if (d == 0) a.part_ml[to] = float2{all, total};
     }
   }
 }
 
-template <int D, bool kFp8, int kWaves>
+template <int D, bool kFp8, int kWaves, bool kParts>
 __global__ void __launch_bounds__(kWaves* kWave, D == 64 ? 4 : 2) k_kv8_attend_narrow(const Attend a) {
   extern __shared__ uint4 dynamic[];
-  narrow_block<D, kFp8, kWaves, true>(a, blockIdx.x, wave_id(), *reinterpret_cast<NarrowShared<D, kWaves>*>(dynamic));
+  narrow_block<D, kFp8, kWaves, true, kParts>(a, blockIdx.x, wave_id(), *reinterpret_cast<NarrowShared<D, kWaves>*>(dynamic));
 }
 
 // ---- many columns: prompt chunks
@@ -1060,11 +1172,6 @@ __device__ __forceinline__ WideTable wide_table(const Attend& a, const int* row,
   if (!inside) x.s = Scales{0.0f, -INFINITY};
   else if (bad || x.s.lv != x.s.lv) x.s = Scales{nan_of(), -INFINITY};
   return x;
-}
-
-__device__ __forceinline__ int uniform_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
-__device__ __forceinline__ float uniform_of(float v, int lane) {
-  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
 }
 
 // A segment of this wave: where its page's head begins in either cache, its
@@ -1274,7 +1381,7 @@ __device__ __forceinline__ WideItem wide_find(const Attend& a, int index, bool w
   WideItem x;
   x.splits = a.wide_splits;
   if (a.requests > 1) {
-    const int free = kWideParts - (int)min((int64_t)kWideParts, (int64_t)others * a.kv * a.narrow_splits / a.narrow_items);
+    const int free = kWideParts - (int)min((int64_t)kWideParts, ((int64_t)others + a.narrow_share) * a.kv / a.narrow_items);
     x.splits = max(1, min(a.wide_splits, free / max(1, total * a.kv)));
   }
   const int h = index % a.kv, item = index / a.kv, rank = whole_tiles ? item : item / x.splits;
@@ -1471,7 +1578,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, Wide<D>::kWaves / 4) k_kv8_
     wide_block<D, kFp8>(a, i, sh.wide);
   } else {
     const int w = wave_id();
-    narrow_block<D, kFp8, 4, false>(a, (i - a.wide_blocks) * (Wide<D>::kWaves / 4) + w / 4, w % 4, sh.narrow[w / 4]);
+    narrow_block<D, kFp8, 4, false, true>(a, (i - a.wide_blocks) * (Wide<D>::kWaves / 4) + w / 4, w % 4, sh.narrow[w / 4]);
   }
 }
 
@@ -1483,6 +1590,7 @@ constexpr int kCombineThreads = 256, kQuarters = 4, kMostShares = 512;  // parts
 struct CombineShared {
   Found found;
   float share[kMostShares];
+  f32x4 sums[kCombineThreads];
 };
 
 // Sum or maximum over a lane's group of 16 or of all 64.
@@ -1520,19 +1628,17 @@ __global__ void __launch_bounds__(kCombineThreads) k_kv8_combine(const Attend a,
     c0 = item.tile * kWideColumns;
     columns = min(kWideColumns, rq.count * a.group - c0);
     const int units = (rq.len + kUnit - 1) / kUnit, per = wide_per(units, item.splits);
-    parts = ((wide_end(a, rq, c0) + kUnit - 1) / kUnit + per - 1) / per;
+    parts = max(1, ((wide_end(a, rq, c0) + kUnit - 1) / kUnit + per - 1) / per);
     from = a.narrow_parts + (size_t)item.part * kWideColumns;
     stride = kWideColumns;
   } else {
-    const int b = index / a.kv;
-    if (a.narrow_splits == 1 || !request_at(a, b, rq) || !rq.narrow) return;
+    NarrowPart part;
+    if (!narrow_find<false>(a, index / a.kv, part, rq) || part.parts == 1) return;
     columns = rq.count * a.group;
-    const int units = (rq.len + kUnit - 1) / kUnit;
-    parts = units > 0 ? (units + narrow_per(units, a.narrow_splits) - 1) / narrow_per(units, a.narrow_splits) : 0;
-    from = ((size_t)b * a.narrow_splits * a.kv + h) * 16;
+    parts = part.parts;
+    from = ((size_t)part.first * a.kv + h) * 16;
     stride = 16 * a.kv;
   }
-  parts = max(parts, 1);  // (the first is there in any case)
   const int mine = wide ? kWideColumns / kQuarters : 16 / kQuarters;
   from += quarter * mine;
   columns = min(columns - quarter * mine, mine);
@@ -1541,25 +1647,41 @@ __global__ void __launch_bounds__(kCombineThreads) k_kv8_combine(const Attend a,
   if (parts <= 16) combine_shares<false>(a.part_ml + from, stride, parts, columns, sh.share);
   else combine_shares<true>(a.part_ml + from, stride, parts, columns, sh.share);
   __syncthreads();
-  const int heads = a.kv * a.group;
-  for (int e = threadIdx.x; e < columns * (D / 4); e += kCombineThreads) {
-    const int c = e / (D / 4), d = 4 * (e % (D / 4));
-    const float* const x = a.part + (from + c) * D + d;
+  // Where the columns leave threads over, those take a share of the parts
+  // each, so that a part's load does not wait for the one eight before it.
+  const int slots = columns * (D / 4), groups = max(1, kCombineThreads / slots);
+  const auto joined = [&](int e, int first) {
+    const float* const x = a.part + (from + e / (D / 4)) * D + 4 * (e % (D / 4));
+    const float* const share = sh.share + e / (D / 4);
     f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
     constexpr int kAhead = 8;
-    for (int p0 = 0; p0 < parts; p0 += kAhead) {
+    for (int p0 = first; p0 < parts; p0 += kAhead * groups) {
       f32x4 y[kAhead];
 #pragma unroll
-      for (int p = 0; p < kAhead; ++p) y[p] = *reinterpret_cast<const f32x4*>(x + (size_t)min(p0 + p, parts - 1) * stride * D);
+      for (int i = 0; i < kAhead; ++i) y[i] = *reinterpret_cast<const f32x4*>(x + (size_t)min(p0 + i * groups, parts - 1) * stride * D);
 #pragma unroll
-      for (int p = 0; p < kAhead; ++p)
-        if (p0 + p < parts) acc += sh.share[(p0 + p) * columns + c] * y[p];
+      for (int i = 0; i < kAhead; ++i)
+        if (p0 + i * groups < parts) acc += share[(p0 + i * groups) * columns] * y[i];
     }
-    const int i = (c0 + c) / a.group, j = c0 + c - i * a.group;
+    return acc;
+  };
+  const auto store = [&](int e, const f32x4& acc) {
+    const int c = c0 + e / (D / 4), i = c / a.group, j = c - i * a.group;
     uint2 y{0, 0};
     if (rq.past + i >= 0) y = uint2{pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3])};
-    *reinterpret_cast<uint2*>(a.out + ((size_t)(rq.row0 + i) * heads + h * a.group + j) * D + d) = y;
+    *reinterpret_cast<uint2*>(a.out + ((size_t)(rq.row0 + i) * (a.kv * a.group) + h * a.group + j) * D + 4 * (e % (D / 4))) = y;
+  };
+  if (groups == 1) {
+    for (int e = threadIdx.x; e < slots; e += kCombineThreads) store(e, joined(e, 0));
+    return;
   }
+  const int t = threadIdx.x, g = t / slots;
+  if (g < groups) sh.sums[t] = joined(t - g * slots, g);
+  __syncthreads();
+  if (t >= slots) return;
+  f32x4 acc = sh.sums[t];
+  for (int i = 1; i < groups; ++i) acc += sh.sums[t + i * slots];
+  store(t, acc);
 }
 
 // ------------------------------------------------------------------ host
@@ -1583,8 +1705,10 @@ bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0
 bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 
 struct Splits {
-  int narrow, wide;     // parts of a request's keys for each kind of request
-  int waves;            // of a narrow block, where there are no wide requests
+  int share, least;     // of the narrow requests' division; 0: not divided
+  int waves;            // of a narrow part
+  int64_t narrow;       // most narrow parts, of all requests
+  int wide;             // parts of a wide tile
   int64_t wide_tiles;   // most tiles that the rows can make
   int64_t wide_blocks;  // and blocks for them
   bool has_wide;
@@ -1595,7 +1719,7 @@ constexpr int kMostWideParts = 16;
 // (the lengths are on the device; the table's width bounds them).
 Splits splits_for(int32_t rows, int32_t requests, int32_t kv, int32_t group, int32_t max_rows, int32_t width, int32_t page,
                   int32_t dim) {
-  Splits s{1, 1, 4, 0, 0, false};
+  Splits s{0, 0, 4, requests, 1, 0, 0, false};
   const int64_t positions = std::min<int64_t>((int64_t)width * page, INT32_MAX), units = (positions + kUnit - 1) / kUnit;
   const auto parts = [&](int64_t wanted, int64_t blocks, int64_t least) {
     return (int)std::max<int64_t>(1, std::min({wanted / blocks, positions / least, (int64_t)kWave}));
@@ -1605,7 +1729,6 @@ Splits splits_for(int32_t rows, int32_t requests, int32_t kv, int32_t group, int
   constexpr int most = 8;
   const int64_t full = dim == 64 ? 4096 : 2048;
   while (s.waves < most && units >= 2 * s.waves && blocks * s.waves < full) s.waves *= 2;
-  s.narrow = parts(full / s.waves, blocks, 128 * s.waves);
   s.has_wide = (int64_t)max_rows * group > 16;
   if (s.has_wide) {
     s.waves = 4;  // beside wide tiles
@@ -1619,17 +1742,23 @@ Splits splits_for(int32_t rows, int32_t requests, int32_t kv, int32_t group, int
       s.wide = (int)std::max<int64_t>(1, std::min<int64_t>(units / kLeastPart, kMostWideParts));
       s.wide_blocks = s.wide > 1 ? std::max<int64_t>(s.wide_tiles * kv, kWideParts) : s.wide_tiles * kv;
     }
-    // The narrow requests beside them are divided only to keep one block's
-    // share to 8,192 positions.
-    s.narrow = (int)std::min<int64_t>({s.narrow, (positions + 8191) / 8192, kWave});
+  }
+  // Where the requests' heads fill half the chip, or more than the parts and
+  // their combination (6 us) cost is in one wave's longest share, only long
+  // contexts are divided.
+  const int64_t target = s.has_wide ? kWideParts : full / s.waves;
+  const bool many = blocks > target / 2;
+  s.least = s.has_wide ? 32 : many ? 128 : s.waves;
+  const int64_t from = s.has_wide ? 96 : many ? 256 : 32;
+  if (requests <= kDivided && units >= from && requests * units <= 1 << 30) {
+    s.share = (int)std::max<int64_t>(1, target / kv);
+    s.narrow = std::min<int64_t>(requests + s.share, requests * ((units + s.least - 1) / s.least));
   }
   return s;
 }
 
 // Columns of the narrow and of the wide parts in the workspace.
-size_t narrow_columns(const Splits& s, int64_t requests, int64_t kv) {
-  return s.narrow > 1 ? (size_t)(requests * kv * s.narrow * 16) : 0;
-}
+size_t narrow_columns(const Splits& s, int64_t kv) { return s.share > 0 ? (size_t)(s.narrow * kv * 16) : 0; }
 size_t wide_columns(const Splits& s) { return s.has_wide && s.wide > 1 ? (size_t)kWideParts * kWideColumns : 0; }
 
 template <int kThreads, int kEach>
@@ -1641,13 +1770,15 @@ void plan(const lfm25_kv8_plan_call& c, int shift, hipStream_t stream) {
 
 template <int D, bool kFp8, int kWaves>
 void attend_narrow(const Attend& a, int64_t blocks, hipStream_t stream) {
-  hipLaunchKernelGGL((k_kv8_attend_narrow<D, kFp8, kWaves>), dim3((unsigned)blocks), dim3(kWaves * kWave),
-                     sizeof(NarrowShared<D, kWaves>), stream, a);
+  const dim3 grid((unsigned)blocks), block(kWaves * kWave);
+  const size_t lds = sizeof(NarrowShared<D, kWaves>);
+  if (a.narrow_share > 0) hipLaunchKernelGGL((k_kv8_attend_narrow<D, kFp8, kWaves, true>), grid, block, lds, stream, a);
+  else hipLaunchKernelGGL((k_kv8_attend_narrow<D, kFp8, kWaves, false>), grid, block, lds, stream, a);
 }
 
 template <int D, bool kFp8>
 int attend(const Attend& a, const Splits& s, hipStream_t stream) {
-  const int64_t narrow = (int64_t)a.requests * a.kv * a.narrow_splits;
+  const int64_t narrow = s.narrow * a.kv;
   if (s.has_wide) {
     hipLaunchKernelGGL((k_kv8_attend_both<D, kFp8>), dim3((unsigned)(a.wide_blocks + a.narrow_blocks)), dim3(Wide<D>::kThreads),
                        sizeof(BothShared<D>), stream, a);
@@ -1656,10 +1787,10 @@ int attend(const Attend& a, const Splits& s, hipStream_t stream) {
   } else {
     attend_narrow<D, kFp8, 8>(a, narrow, stream);
   }
-  if (s.narrow > 1 || (s.has_wide && s.wide > 1)) {
+  if (s.share > 0 || (s.has_wide && s.wide > 1)) {
     // (a tile in parts is one of at most kWideParts / 2)
     const int wide_items = s.has_wide && s.wide > 1 ? kWideParts / 2 : 0;
-    const int64_t narrow_items = s.narrow > 1 ? (int64_t)a.requests * a.kv : 0;
+    const int64_t narrow_items = s.share > 0 ? (int64_t)a.requests * a.kv : 0;
     hipLaunchKernelGGL((k_kv8_combine<D>), dim3((unsigned)((wide_items + narrow_items) * kQuarters)), dim3(kCombineThreads), 0, stream, a, wide_items);
   }
   return check_launch("lfm25_kv8_attention");
@@ -1746,7 +1877,7 @@ extern "C" size_t lfm25_kv8_attention_workspace_bytes(int32_t rows, int32_t head
       !attend_shape(rows, heads, kv_heads, requests, max_rows, width, page))
     return 0;
   const Splits s = splits_for(rows, requests, kv_heads, heads / kv_heads, std::min(max_rows, rows), width, page, head_dim);
-  return 4 * (narrow_columns(s, requests, kv_heads) + wide_columns(s)) * (head_dim + 2);
+  return 4 * (narrow_columns(s, kv_heads) + wide_columns(s)) * (head_dim + 2);
 }
 
 extern "C" int lfm25_kv8_attention(const lfm25_kv8_attention_call* call, lfm25_stream_t stream) {
@@ -1768,7 +1899,7 @@ extern "C" int lfm25_kv8_attention(const lfm25_kv8_attention_call* call, lfm25_s
   LFM25_REQUIRE(c.reserved == 0, "lfm25_kv8_attention: reserved must be 0");
   const int group = c.heads / c.kv_heads, max_rows = std::min(c.max_rows, c.rows);
   const Splits s = splits_for(c.rows, c.requests, c.kv_heads, group, max_rows, c.width, c.page, c.head_dim);
-  const size_t columns = narrow_columns(s, c.requests, c.kv_heads) + wide_columns(s);
+  const size_t columns = narrow_columns(s, c.kv_heads) + wide_columns(s);
   LFM25_REQUIRE(columns == 0 || (c.workspace != nullptr && aligned16(c.workspace)),
                 "lfm25_kv8_attention: needs a 16-byte aligned workspace of lfm25_kv8_attention_workspace_bytes()");
   Attend a{};
@@ -1779,15 +1910,15 @@ extern "C" int lfm25_kv8_attention(const lfm25_kv8_attention_call* call, lfm25_s
   a.out = c.output;
   a.part = static_cast<float*>(c.workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part + columns * c.head_dim);
-  a.narrow_parts = narrow_columns(s, c.requests, c.kv_heads);
+  a.narrow_parts = narrow_columns(s, c.kv_heads);
   a.status = c.status;
   a.width = c.width, a.rows = c.rows, a.kv = c.kv_heads, a.group = group, a.pages = c.pages, a.shift = page_shift(c.page);
   a.requests = c.requests, a.max_rows = max_rows;
-  a.narrow_splits = s.narrow, a.wide_splits = s.wide;
+  a.narrow_share = s.share, a.narrow_least = s.least, a.wide_splits = s.wide;
   a.wide_blocks = (int)s.wide_blocks;
   a.early_blocks = std::min(a.wide_blocks, kWideParts);
   a.narrow_items = (c.head_dim == 64 ? Wide<64>::kWaves : Wide<128>::kWaves) / 4;
-  a.narrow_blocks = (int)(((int64_t)c.requests * c.kv_heads * s.narrow + a.narrow_items - 1) / a.narrow_items);
+  a.narrow_blocks = (int)((s.narrow * c.kv_heads + a.narrow_items - 1) / a.narrow_items);
   a.scale = c.scale * 1.4426950408889634f;
   if (c.head_dim == 64) return c.format == LFM25_KV8_FP8 ? attend<64, true>(a, s, stream) : attend<64, false>(a, s, stream);
   return c.format == LFM25_KV8_FP8 ? attend<128, true>(a, s, stream) : attend<128, false>(a, s, stream);

@@ -339,6 +339,36 @@ def test_attention_over_long_contexts(gpu, lab, dtype, counts, dim, group):
     check_attention(lab.ops, make_case(1, [9000, 130], counts, 1, group, dim, 128, dtype, width=600))
 
 
+@pytest.mark.parametrize("n,kv,dim", [(3, 2, 64), (64, 1, 64), (65, 1, 64), (200, 1, 64), (256, 1, 128), (257, 1, 64), (130, 2, 128)])
+def test_attention_of_batches_of_uneven_lengths(gpu, lab, n, kv, dim):
+    """One long context, short ones, requests that rest and one past its table, in parts found on the device."""
+    rng = np.random.default_rng(n)
+    past = rng.integers(0, 90, n)
+    past[[0, n // 2, n - 1]] = [4000, 700, 2300]
+    counts = rng.integers(1, 3, n)
+    counts[1::7] = 0
+    c = make_case(n, past, counts, kv, 2, dim, 32, torch.float8_e4m3fn, width=130)
+    check_attention(lab.ops, c)
+    k, v, ks, vs = host_cache(c["cache"])
+    want, reach = plain.attention(c["q"].double().cpu().numpy(), k, v, ks, vs, host(c["table"]), past, host(c["starts"]), dim ** -0.5)
+    starts, moved = host(c["starts"]), past.copy()
+    moved[n // 2] = 5000  # past the table: NaN there, the others as before
+    status = ints([0])
+    got = attend(lab.ops, c, status, past=ints(moved)).double().cpu().numpy()
+    mine = slice(starts[n // 2], starts[n // 2 + 1])
+    assert np.isnan(got[mine]).all() and host(status)[0] == (lab.ops.KV8_BAD_PAGE if counts[n // 2] else 0)
+    keep = np.ones(len(got), bool)
+    keep[mine] = False
+    assert (np.abs(got - want)[keep] <= reach[keep]).all()
+
+
+def test_attention_of_long_contexts_beside_prompts(gpu, lab):
+    for dim, n in ((64, 20), (128, 5), (64, 70)):
+        past, counts = [60 * b for b in range(n)], [1] * n
+        past[3], counts[1], counts[2], counts[n - 1] = 7000, 150, 0, 40
+        check_attention(lab.ops, make_case(n, past, counts, 2, 2, dim, 64, torch.int8))
+
+
 @pytest.mark.parametrize("counts", [[1, 1], [30, 30]])
 def test_attention_of_peaked_and_flat_scores(gpu, lab, counts):
     for stretch, scale in ((40.0, 0.125), (1.0, 0.0), (1e-3, 1.0), (3e4, 2.0)):

@@ -99,8 +99,8 @@ def test_workspace_sizes(lab):
     column = 4 * (64 + 2)
     assert size(4, 16, 8, 64, 4, 1, 3, 64) == 0            # too few positions to divide
     assert size(64, 16, 8, 64, 0, 1, 64, 64) == 0          # a refused call
-    assert size(4, 16, 8, 64, 4, 1, 64, 64) == 4 * 8 * 4 * 16 * column            # four parts of 1,024 positions
-    assert size(1, 16, 8, 64, 1, 1, 1 << 20, 64) == 8 * 64 * 16 * column          # 64 parts at most
+    assert size(4, 16, 8, 64, 4, 1, 64, 64) == 32 * 8 * 16 * column                # parts of 512 positions
+    assert size(1, 16, 8, 64, 1, 1, 1 << 20, 64) == 8 * 65 * 16 * column          # a full chip
     assert size(512, 16, 8, 64, 2, 256, 64, 64) == 256 * 128 * column             # parts of tiles of 128 columns
 
 
