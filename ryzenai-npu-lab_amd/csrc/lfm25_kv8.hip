@@ -702,16 +702,12 @@ __device__ __forceinline__ bf16x8 codes8(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(bf16x8, r);
 }
 
-// max(a, b) as the median with infinity, one instruction: fmaxf() quiets each
-// operand first, since the matrix cores' results may be anything (and does so
-// here too, if the compiler sees that it is infinity). A NaN is left out
-// beside a number; two give infinity, whose column is NaN as well.
-__device__ __forceinline__ float hidden_infinity() {
-  float x = INFINITY;
-  asm("" : "+v"(x));
-  return x;
+// The largest of three, one instruction; NaN if one is (the column is NaN
+// then in any case), so that no operand has to be quieted first, as fmaxf()
+// does with the matrix cores' results.
+__device__ __forceinline__ float largest(float a, float b, float c) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
-__device__ __forceinline__ float max_of(float a, float b, float infinity) { return __builtin_amdgcn_fmed3f(a, b, infinity); }
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float nan_of() { return __uint_as_float(0x7fc00000u); }
 
@@ -1018,7 +1014,7 @@ __device__ __forceinline__ void narrow_block(const Attend& a, int index, int w, 
     }
     float most = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) most = fmaxf(most, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
+    for (int t = 0; t < 4; ++t) most = largest(most, s[t][0], largest(s[t][1], s[t][2], s[t][3]));
     // (a segment that the column sees nothing of has -inf here, whatever its scale)
     most = across_max16(most == -INFINITY ? most : most * sc.ks);
     const float new_top = fmaxf(top, across_max16(sc.lv));
@@ -1281,15 +1277,13 @@ __device__ __forceinline__ void wide_unit(const WideStages<D>& sh, int first, in
       for (int i = 0; i < 16; ++i)
         if (32 * t + 16 * (i / 8) + i % 8 > behind) s.t[t][i] = -INFINITY;
   }
-  const float infinity = hidden_infinity();
   float most = -INFINITY;
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float v = s.t[t][8 * e];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) v = max_of(v, s.t[t][8 * e + i], infinity);
+      const auto at = [&](int i) { return s.t[t][8 * e + i]; };
+      const float v = largest(largest(at(0), at(1), at(2)), largest(at(3), at(4), at(5)), __builtin_elementwise_maximum(at(6), at(7)));
       // (where the column sees nothing of the segment: -inf, whatever its scale)
       most = fmaxf(most, kMasked && v == -INFINITY ? v : v * sc[2 * t + e].ks);
     }
