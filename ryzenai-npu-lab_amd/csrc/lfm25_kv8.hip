@@ -1162,18 +1162,30 @@ struct WideTable {
   int id;     // page that may be read
   Scales s;
 };
+struct WideEntry {  // as read
+  int id;
+  bool inside, bad;
+  float ks, vs;
+};
 
-__device__ __forceinline__ WideTable wide_table(const Attend& a, const int* row, int h, int64_t at, int end) {
-  const bool inside = at < end;
-  const int entry = inside ? row[at >> a.shift] : 0;
-  const bool bad = (uint32_t)entry >= (uint32_t)a.pages;
-  if (bad && inside) raise(a.status, kStatusPage);
+__device__ __forceinline__ WideEntry wide_entry(const Attend& a, const int* row, int h, int64_t at, int end) {
+  WideEntry e;
+  e.inside = at < end;
+  e.id = e.inside ? row[at >> a.shift] : 0;
+  e.bad = (uint32_t)e.id >= (uint32_t)a.pages;
+  e.id = e.bad ? 0 : e.id;
+  const size_t head = (size_t)e.id * a.kv + h;
+  e.ks = a.ks[head];
+  e.vs = a.vs[head];
+  return e;
+}
+__device__ __forceinline__ WideTable wide_table(const Attend& a, const WideEntry& e) {
+  if (e.bad && e.inside) raise(a.status, kStatusPage);
   WideTable x;
-  x.id = bad ? 0 : entry;
-  const size_t head = (size_t)x.id * a.kv + h;
-  x.s = Scales{a.ks[head] * a.scale, scale_log2(a.vs[head])};
-  if (!inside) x.s = Scales{0.0f, -INFINITY};
-  else if (bad || x.s.lv != x.s.lv) x.s = Scales{nan_of(), -INFINITY};
+  x.id = e.id;
+  x.s = Scales{e.ks * a.scale, scale_log2(e.vs)};
+  if (!e.inside) x.s = Scales{0.0f, -INFINITY};
+  else if (e.bad || x.s.lv != x.s.lv) x.s = Scales{nan_of(), -INFINITY};
   return x;
 }
 
@@ -1350,9 +1362,38 @@ struct WideItem {
 
 __device__ __forceinline__ int wide_per(int units, int splits) { return max((units + splits - 1) / splits, kLeastPart); }
 
-// Item `index` (head first) of the block, b < 0 if there is none.
+// How many parts each tile is divided into, with `tiles` of them and `others`
+// narrow requests.
+__device__ __forceinline__ int wide_splits(const Attend& a, int tiles, int others) {
+  if (a.requests == 1) return a.wide_splits;
+  const int free = kWideParts - (int)min((int64_t)kWideParts, ((int64_t)others + a.narrow_share) * a.kv / a.narrow_items);
+  return max(1, min(a.wide_splits, free / max(1, tiles * a.kv)));
+}
+
+// Item `index` (head first) of the block, b < 0 if there is none. Up to 64
+// requests are a lane's each, and every wave finds the item for itself;
+// more are looked through by the whole block.
 template <int kThreads>
-__device__ __forceinline__ WideItem wide_find(const Attend& a, int index, bool whole_tiles, Found& sh) {
+__device__ __forceinline__ WideItem wide_find(const Attend& a, int index, bool whole_tiles, Request& rq, Found& sh) {
+  const int h = index % a.kv, item = index / a.kv;
+  WideItem x;
+  if (a.requests <= kWave) {
+    Request my;
+    const bool here = lane_id() < a.requests && request_at(a, lane_id(), my);
+    const int n = here && !my.narrow ? (my.count * a.group + kWideColumns - 1) / kWideColumns : 0;
+    const int upto = wave_sums(n), total = uniform_of(upto, kWave - 1);
+    x.splits = wide_splits(a, total, __builtin_popcountll(__ballot(n == 0 && lane_id() < a.requests)));
+    const int rank = whole_tiles ? item : item / x.splits;
+    x.sp = whole_tiles ? 0 : item - rank * x.splits;
+    x.part = (rank * a.kv + h) * x.splits + x.sp;
+    const uint64_t reach = __ballot(upto > rank);
+    x.b = reach ? __builtin_ctzll(reach) : -1;
+    const int lane = max(x.b, 0);
+    x.tile = uniform_of(upto, lane) - 1 - rank;
+    rq.row0 = uniform_of(my.row0, lane), rq.count = uniform_of(my.count, lane), rq.past = uniform_of(my.past, lane);
+    rq.len = uniform_of(my.len, lane), rq.cap = clamp_int((int64_t)a.width << a.shift);
+    return x;
+  }
   const int each = (a.requests + kThreads - 1) / kThreads, b0 = threadIdx.x * each;
   const int l = lane_id(), w = wave_id();
   const auto tiles_of = [&](int b) {
@@ -1379,13 +1420,8 @@ __device__ __forceinline__ WideItem wide_find(const Attend& a, int index, bool w
     total += sh.waves[i];
     others += sh.few[i];
   }
-  WideItem x;
-  x.splits = a.wide_splits;
-  if (a.requests > 1) {
-    const int free = kWideParts - (int)min((int64_t)kWideParts, ((int64_t)others + a.narrow_share) * a.kv / a.narrow_items);
-    x.splits = max(1, min(a.wide_splits, free / max(1, total * a.kv)));
-  }
-  const int h = index % a.kv, item = index / a.kv, rank = whole_tiles ? item : item / x.splits;
+  x.splits = wide_splits(a, total, others);
+  const int rank = whole_tiles ? item : item / x.splits;
   x.sp = whole_tiles ? 0 : item - rank * x.splits;
   x.part = (rank * a.kv + h) * x.splits + x.sp;
   int first = upto - mine;
@@ -1402,6 +1438,7 @@ __device__ __forceinline__ WideItem wide_find(const Attend& a, int index, bool w
   __syncthreads();
   x.b = __builtin_amdgcn_readfirstlane(sh.request);
   x.tile = __builtin_amdgcn_readfirstlane(sh.tile);
+  if (x.b >= 0) request_at(a, x.b, rq);
   return x;
 }
 
@@ -1415,10 +1452,9 @@ __device__ __forceinline__ int wide_end(const Attend& a, const Request& rq, int 
 template <int D, bool kFp8>
 __device__ __forceinline__ void wide_block(const Attend& a, int index, WideShared<D>& sh) {
   const int h = index % a.kv, w = wave_id(), l = lane_id();
-  const WideItem item = wide_find<Wide<D>::kThreads>(a, index, false, sh.found);
-  if (item.b < 0) return;
   Request rq;
-  if (!request_at(a, item.b, rq)) return;
+  const WideItem item = wide_find<Wide<D>::kThreads>(a, index, false, rq, sh.found);
+  if (item.b < 0) return;
   const int* row = a.table + (size_t)item.b * a.width;
   const int columns = rq.count * a.group, c0 = item.tile * kWideColumns, end = wide_end(a, rq, c0);
   const int units = (rq.len + kUnit - 1) / kUnit, per = wide_per(units, item.splits);
@@ -1432,25 +1468,31 @@ __device__ __forceinline__ void wide_block(const Attend& a, int index, WideShare
   const uint32_t page_bytes = (uint32_t)((a.kv << a.shift) * D), head_bytes = (uint32_t)((h << a.shift) * D);
   const uint32_t k_lane = (uint32_t)((l >> 2) * D + 16 * (l & 3)), v_lane = (uint32_t)(l << a.shift);
   const int in_page = (1 << a.shift) - 1;
-  WideTable table = wide_table(a, row, h, (int64_t)first + kRound * l, end);
-  WideUnit<D> next;
+  const WideEntry entry = wide_entry(a, row, h, (int64_t)first + kRound * l, end);
+  WideTable table;
+  table.id = entry.id;
+  WideUnit<D> now, next;
   // Loads are made for rounds past the last too (of page 0; never used).
-  const auto load_keys = [&](int i) {
-    if (i > 0 && i % kWave == 0) table = wide_table(a, row, h, (int64_t)first + (int64_t)kRound * (i + l), end);
-    next.of_v = next.of_k;
-    next.of_k.region = (size_t)(uint32_t)uniform_of(table.id, i % kWave) * page_bytes + head_bytes;
-    next.of_k.s = Scales{uniform_of(table.s.ks, i % kWave), uniform_of(table.s.lv, i % kWave)};
-    next.of_k.at = first + kRound * i;
-    const uint8_t* const k = a.k + (next.of_k.region + (uint32_t)(next.of_k.at & in_page) * D);
+  const auto load_keys = [&](int i, WideUnit<D>& x) {
+    x.of_k.region = (size_t)(uint32_t)uniform_of(table.id, i % kWave) * page_bytes + head_bytes;
+    x.of_k.at = first + kRound * i;
+    const uint8_t* const k = a.k + (x.of_k.region + (uint32_t)(x.of_k.at & in_page) * D);
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) next.k[c] = *reinterpret_cast<const uint4*>(k + (k_lane + 64 * c));
+    for (int c = 0; c < D / 64; ++c) x.k[c] = *reinterpret_cast<const uint4*>(k + (k_lane + 64 * c));
+  };
+  const auto scale_keys = [&](int i, WideUnit<D>& x) {
+    x.of_k.s = Scales{uniform_of(table.s.ks, i % kWave), uniform_of(table.s.lv, i % kWave)};
   };
   const auto load_values = [&] {
     const uint8_t* const v = a.v + (next.of_v.region + (uint32_t)(next.of_v.at & in_page));
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) next.v[c] = *reinterpret_cast<const uint4*>(v + (v_lane + (uint32_t)((64 * c) << a.shift)));
   };
-  load_keys(0);
+  // all that the first round needs, before anything is waited for
+  load_keys(0, now);
+  load_keys(1, next);
+  next.of_v = now.of_k;
+  load_values();
   const int half = l >> 5;
   const int column = c0 + 32 * w4 + (l & 31);
   const bool live = column < columns;
@@ -1483,7 +1525,11 @@ __device__ __forceinline__ void wide_block(const Attend& a, int index, WideShare
   // (matrix and LDS work): one group is in the first half while the other is
   // in the second, a barrier apart. Keys are staged a round ahead of values.
   const auto load = [&](int i) {  // keys of round i + 1, values of round i
-    load_keys(i + 1);
+    ++i;
+    if (i % kWave == 0) table = wide_table(a, wide_entry(a, row, h, (int64_t)first + (int64_t)kRound * (i + l), end));
+    next.of_v = next.of_k;
+    load_keys(i, next);
+    scale_keys(i, next);
     load_values();
   };
   const auto store = [&](int i) {
@@ -1498,8 +1544,11 @@ __device__ __forceinline__ void wide_block(const Attend& a, int index, WideShare
     load(i + 2);
     lds_barrier();
   };
-  store_keys<D, kFp8>(mine, w4, 0, next);
-  load(0);
+  table = wide_table(a, entry);
+  scale_keys(0, now);
+  next.of_v.s = now.of_k.s;
+  scale_keys(1, next);
+  store_keys<D, kFp8>(mine, w4, 0, now);
   if (group & 1) lds_barrier();
   stage(-1);
   int i = 0;
@@ -1624,8 +1673,8 @@ __global__ void __launch_bounds__(kCombineThreads) k_kv8_combine(const Attend a,
   int parts, columns, c0 = 0, stride;  // columns of the item, the first of this block's
   size_t from;  // column 0 of part 0
   if (wide) {
-    const WideItem item = wide_find<kCombineThreads>(a, index, true, sh.found);
-    if (item.b < 0 || item.splits == 1 || !request_at(a, item.b, rq)) return;
+    const WideItem item = wide_find<kCombineThreads>(a, index, true, rq, sh.found);
+    if (item.b < 0 || item.splits == 1) return;
     c0 = item.tile * kWideColumns;
     columns = min(kWideColumns, rq.count * a.group - c0);
     const int units = (rq.len + kUnit - 1) / kUnit, per = wide_per(units, item.splits);
