@@ -1694,21 +1694,27 @@ __global__ void __launch_bounds__(kCombineThreads) k_kv8_combine(const Attend a,
   columns = min(columns - quarter * mine, mine);
   c0 += quarter * mine;
   if (columns <= 0) return;
+  // Where the columns leave threads over, those take a share of the parts
+  // each, so that a part's load does not wait for the one eight before it. The
+  // first loads are on their way while the shares are made.
+  const int t = threadIdx.x, slots = columns * (D / 4), groups = max(1, kCombineThreads / slots), g = groups == 1 ? 0 : t / slots;
+  constexpr int kAhead = 8;
+  const auto fetch = [&](int e, int p0, f32x4 (&y)[kAhead]) {
+    const float* const x = a.part + (from + e / (D / 4)) * D + 4 * (e % (D / 4));
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) y[i] = *reinterpret_cast<const f32x4*>(x + (size_t)min(p0 + i * groups, parts - 1) * stride * D);
+  };
+  const int e0 = t - g * slots;
+  f32x4 ready[kAhead];
+  fetch(min(e0, slots - 1), min(g, parts - 1), ready);
   if (parts <= 16) combine_shares<false>(a.part_ml + from, stride, parts, columns, sh.share);
   else combine_shares<true>(a.part_ml + from, stride, parts, columns, sh.share);
   __syncthreads();
-  // Where the columns leave threads over, those take a share of the parts
-  // each, so that a part's load does not wait for the one eight before it.
-  const int slots = columns * (D / 4), groups = max(1, kCombineThreads / slots);
-  const auto joined = [&](int e, int first) {
-    const float* const x = a.part + (from + e / (D / 4)) * D + 4 * (e % (D / 4));
+  const auto joined = [&](int e, f32x4 (&y)[kAhead]) {
     const float* const share = sh.share + e / (D / 4);
     f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int kAhead = 8;
-    for (int p0 = first; p0 < parts; p0 += kAhead * groups) {
-      f32x4 y[kAhead];
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) y[i] = *reinterpret_cast<const f32x4*>(x + (size_t)min(p0 + i * groups, parts - 1) * stride * D);
+    for (int p0 = g; p0 < parts; p0 += kAhead * groups) {
+      if (p0 != g) fetch(e, p0, y);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
         if (p0 + i * groups < parts) acc += share[(p0 + i * groups) * columns] * y[i];
@@ -1722,11 +1728,13 @@ __global__ void __launch_bounds__(kCombineThreads) k_kv8_combine(const Attend a,
     *reinterpret_cast<uint2*>(a.out + ((size_t)(rq.row0 + i) * (a.kv * a.group) + h * a.group + j) * D + 4 * (e % (D / 4))) = y;
   };
   if (groups == 1) {
-    for (int e = threadIdx.x; e < slots; e += kCombineThreads) store(e, joined(e, 0));
+    for (int e = t; e < slots; e += kCombineThreads) {
+      if (e != t) fetch(e, 0, ready);
+      store(e, joined(e, ready));
+    }
     return;
   }
-  const int t = threadIdx.x, g = t / slots;
-  if (g < groups) sh.sums[t] = joined(t - g * slots, g);
+  if (g < groups) sh.sums[t] = joined(e0, ready);
   __syncthreads();
   if (t >= slots) return;
   f32x4 acc = sh.sums[t];
