@@ -622,6 +622,7 @@ struct Attend {
   int narrow_least;  // least units of a part
   int wide_splits, wide_blocks, early_blocks, narrow_blocks;
   int narrow_items;     // of a block, beside wide tiles
+  int narrow_columns;   // a request of at most so many is narrow
   size_t narrow_parts;  // columns of the narrow parts in `part`
   float scale;  // log2(e) * the softmax scale
 };
@@ -652,7 +653,7 @@ __device__ __forceinline__ bool request_at(const Attend& a, int b, Request& r) {
   const int64_t len = (int64_t)r.past + r.count;
   r.past = min(r.past, INT32_MAX - r.count);  // (past any table either way; positions stay ints)
   r.len = len < 0 ? 0 : len > r.cap ? r.cap : (int)len;
-  r.narrow = (int64_t)r.count * a.group <= 16;
+  r.narrow = (int64_t)r.count * a.group <= a.narrow_columns;
   if (len > r.cap) raise(a.status, kStatusPage);
   return true;
 }
@@ -1399,7 +1400,7 @@ __device__ __forceinline__ WideItem wide_find(const Attend& a, int index, bool w
   const auto tiles_of = [&](int b) {
     if (b >= a.requests) return 0;
     const int s0 = a.starts[b], s1 = a.starts[b + 1];
-    if (s0 < 0 || s1 <= s0 || s1 > a.rows || s1 - s0 > a.max_rows || (int64_t)(s1 - s0) * a.group <= 16) return 0;
+    if (s0 < 0 || s1 <= s0 || s1 > a.rows || s1 - s0 > a.max_rows || (int64_t)(s1 - s0) * a.group <= a.narrow_columns) return 0;
     return (int)(((int64_t)(s1 - s0) * a.group + kWideColumns - 1) / kWideColumns);
   };
   int mine = 0, few = 0;  // tiles, and requests that have none
@@ -1610,25 +1611,35 @@ __device__ __forceinline__ void wide_block(const Attend& a, int index, WideShare
 // Wide tiles first, since they take longest, then the narrow requests. (LDS
 // as dynamic memory: a static array past half of a CU's makes the compiler
 // plan for 512 registers and move results between their two halves.)
-template <int D>
+//
+// kItems: narrow items of a block, 0 for a launch without any, 1 where there
+// are few of them (each then has all of the block's waves).
+template <int D, int kItems>
 union BothShared {
   WideShared<D> wide;
-  NarrowShared<D, 4> narrow[Wide<D>::kWaves / 4];
+  NarrowShared<D, kItems == 1 ? Wide<D>::kWaves : 4> narrow[kItems > 0 ? kItems : 1];
 };
 
-template <int D, bool kFp8>
+template <int D, bool kFp8, int kItems>
 __global__ void __launch_bounds__(Wide<D>::kThreads, Wide<D>::kWaves / 4) k_kv8_attend_both(const Attend a) {
   extern __shared__ uint4 dynamic[];
-  BothShared<D>& sh = *reinterpret_cast<BothShared<D>*>(dynamic);
-  // wide tiles first, since they take longest; those past the first round of
-  // the chip, which may be none, behind the narrow requests
+  BothShared<D, kItems>& sh = *reinterpret_cast<BothShared<D, kItems>*>(dynamic);
+  if constexpr (kItems == 0) {
+    wide_block<D, kFp8>(a, blockIdx.x, sh.wide);
+    return;
+  }
+  // The first `early_blocks` are tiles, since they take longest; those past
+  // the first round of the chip, which may be none, come behind the narrow
+  // requests. (Divided tiles are short: then the narrow requests come first.)
   int i = blockIdx.x;
   if (i >= a.early_blocks) i = i < a.early_blocks + a.narrow_blocks ? i + (a.wide_blocks - a.early_blocks) : i - a.narrow_blocks;
   if (i < a.wide_blocks) {
     wide_block<D, kFp8>(a, i, sh.wide);
+  } else if constexpr (kItems == 1) {
+    narrow_block<D, kFp8, Wide<D>::kWaves, true, true>(a, i - a.wide_blocks, wave_id(), sh.narrow[0]);
   } else {
     const int w = wave_id();
-    narrow_block<D, kFp8, 4, false, true>(a, (i - a.wide_blocks) * (Wide<D>::kWaves / 4) + w / 4, w % 4, sh.narrow[w / 4]);
+    narrow_block<D, kFp8, 4, false, true>(a, (i - a.wide_blocks) * kItems + w / 4, w % 4, sh.narrow[w / 4]);
   }
 }
 
@@ -1765,11 +1776,13 @@ bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0
 struct Splits {
   int share, least;     // of the narrow requests' division; 0: not divided
   int waves;            // of a narrow part
+  int items;            // of a block beside tiles; 0: one request, wide whatever it brings
   int64_t narrow;       // most narrow parts, of all requests
   int wide;             // parts of a wide tile
   int64_t wide_tiles;   // most tiles that the rows can make
   int64_t wide_blocks;  // and blocks for them
   bool has_wide;
+  bool few_tiles;       // about half as many as the chip has room for, or fewer
 };
 constexpr int kMostWideParts = 16;
 
@@ -1777,7 +1790,7 @@ constexpr int kMostWideParts = 16;
 // (the lengths are on the device; the table's width bounds them).
 Splits splits_for(int32_t rows, int32_t requests, int32_t kv, int32_t group, int32_t max_rows, int32_t width, int32_t page,
                   int32_t dim) {
-  Splits s{0, 0, 4, requests, 1, 0, 0, false};
+  Splits s{0, 0, 4, 1, requests, 1, 0, 0, false, false};
   const int64_t positions = std::min<int64_t>((int64_t)width * page, INT32_MAX), units = (positions + kUnit - 1) / kUnit;
   const auto parts = [&](int64_t wanted, int64_t blocks, int64_t least) {
     return (int)std::max<int64_t>(1, std::min({wanted / blocks, positions / least, (int64_t)kWave}));
@@ -1791,24 +1804,30 @@ Splits splits_for(int32_t rows, int32_t requests, int32_t kv, int32_t group, int
   if (s.has_wide) {
     s.waves = 4;  // beside wide tiles
     const int64_t columns = (int64_t)rows * group;
-    s.wide_tiles = columns / kWideColumns + std::min<int64_t>(requests, columns / 17 + 1);
-    if (requests == 1) {
-      s.wide_tiles = (columns + kWideColumns - 1) / kWideColumns;
-      s.wide = (int)std::min<int64_t>(parts(kWideParts, s.wide_tiles * kv, kLeastPart * kUnit), kMostWideParts);
-      s.wide_blocks = s.wide_tiles * kv * s.wide;
-    } else {
-      s.wide = (int)std::max<int64_t>(1, std::min<int64_t>(units / kLeastPart, kMostWideParts));
-      s.wide_blocks = s.wide > 1 ? std::max<int64_t>(s.wide_tiles * kv, kWideParts) : s.wide_tiles * kv;
+    s.wide_tiles = requests == 1 ? (columns + kWideColumns - 1) / kWideColumns
+                                 : columns / kWideColumns + std::min<int64_t>(requests, columns / 17 + 1);
+    s.few_tiles = columns * kv <= (int64_t)kWideParts / 2 * kWideColumns;  // about; less than half a chip
+    // A tile takes 7 us and 0.8 for each unit, parts and their combination 5
+    // (one tile a head: 13.9 us whole and 16.4 in parts over 512 positions,
+    // 19.7 and 16.8 over 1,024; 21.2 and 17.6 beside single tokens).
+    if (s.few_tiles && units >= 16) {
+      s.wide = requests == 1 ? parts(kWideParts, s.wide_tiles * kv, kLeastPart * kUnit) : (int)(units / kLeastPart);
+      s.wide = std::min(s.wide, kMostWideParts);
     }
+    s.wide_blocks = s.wide_tiles * kv;
+    if (s.wide > 1) s.wide_blocks = requests == 1 ? s.wide_blocks * s.wide : std::max<int64_t>(s.wide_blocks, kWideParts);
+    s.items = requests == 1 ? 0 : s.few_tiles && requests * kv <= 128 ? 1 : (dim == 64 ? Wide<64>::kWaves : Wide<128>::kWaves) / 4;
   }
-  // Where the requests' heads fill half the chip, or more than the parts and
-  // their combination (6 us) cost is in one wave's longest share, only long
-  // contexts are divided.
+  // Single tokens: a unit takes one block 0.2 us (dim 64), and the chip's
+  // memory 0.0016 for each block; parts and their combination 4 (8 requests
+  // of 8 heads: 16.1 us whole and 15.4 in parts over 2,560 positions, 22.1 and
+  // 16.7 over 4,096; 24 requests 24.6 and 29.2). Where the memory bounds it,
+  // still in parts over long contexts, since a batch's lengths may differ.
   const int64_t target = s.has_wide ? kWideParts : full / s.waves;
   const bool many = blocks > target / 2;
   s.least = s.has_wide ? 32 : many ? 128 : s.waves;
-  const int64_t from = s.has_wide ? 96 : many ? 256 : 32;
-  if (requests <= kDivided && units >= from && requests * units <= 1 << 30) {
+  const int64_t from = s.has_wide ? 96 : many ? 256 : units * (dim / 64) * (120 - blocks) >= 2400 ? 2 * s.least : 96;
+  if ((!s.has_wide || requests > 1) && requests <= kDivided && units >= from && requests * units <= 1 << 30) {
     s.share = (int)std::max<int64_t>(1, target / kv);
     s.narrow = std::min<int64_t>(requests + s.share, requests * ((units + s.least - 1) / s.least));
   }
@@ -1834,12 +1853,19 @@ void attend_narrow(const Attend& a, int64_t blocks, hipStream_t stream) {
   else hipLaunchKernelGGL((k_kv8_attend_narrow<D, kFp8, kWaves, false>), grid, block, lds, stream, a);
 }
 
+template <int D, bool kFp8, int kItems>
+void attend_both(const Attend& a, hipStream_t stream) {
+  hipLaunchKernelGGL((k_kv8_attend_both<D, kFp8, kItems>), dim3((unsigned)(a.wide_blocks + a.narrow_blocks)), dim3(Wide<D>::kThreads),
+                     sizeof(BothShared<D, kItems>), stream, a);
+}
+
 template <int D, bool kFp8>
 int attend(const Attend& a, const Splits& s, hipStream_t stream) {
   const int64_t narrow = s.narrow * a.kv;
   if (s.has_wide) {
-    hipLaunchKernelGGL((k_kv8_attend_both<D, kFp8>), dim3((unsigned)(a.wide_blocks + a.narrow_blocks)), dim3(Wide<D>::kThreads),
-                       sizeof(BothShared<D>), stream, a);
+    if (s.items == 0) attend_both<D, kFp8, 0>(a, stream);
+    else if (s.items == 1) attend_both<D, kFp8, 1>(a, stream);
+    else attend_both<D, kFp8, Wide<D>::kWaves / 4>(a, stream);
   } else if (s.waves == 4) {
     attend_narrow<D, kFp8, 4>(a, narrow, stream);
   } else {
@@ -1980,9 +2006,10 @@ extern "C" int lfm25_kv8_attention(const lfm25_kv8_attention_call* call, lfm25_s
   a.requests = c.requests, a.max_rows = max_rows;
   a.narrow_share = s.share, a.narrow_least = s.least, a.wide_splits = s.wide;
   a.wide_blocks = (int)s.wide_blocks;
-  a.early_blocks = std::min(a.wide_blocks, kWideParts);
-  a.narrow_items = (c.head_dim == 64 ? Wide<64>::kWaves : Wide<128>::kWaves) / 4;
-  a.narrow_blocks = (int)((s.narrow * c.kv_heads + a.narrow_items - 1) / a.narrow_items);
+  a.early_blocks = s.wide > 1 && s.few_tiles ? 0 : std::min(a.wide_blocks, kWideParts);
+  a.narrow_items = std::max(1, s.items);
+  a.narrow_blocks = s.items == 0 ? 0 : (int)((s.narrow * c.kv_heads + s.items - 1) / s.items);
+  a.narrow_columns = s.has_wide && s.items == 0 ? 0 : 16;
   a.scale = c.scale * 1.4426950408889634f;
   if (c.head_dim == 64) return c.format == LFM25_KV8_FP8 ? attend<64, true>(a, s, stream) : attend<64, false>(a, s, stream);
   return c.format == LFM25_KV8_FP8 ? attend<128, true>(a, s, stream) : attend<128, false>(a, s, stream);

@@ -363,7 +363,7 @@ def test_attention_of_batches_of_uneven_lengths(gpu, lab, n, kv, dim):
 
 
 def test_attention_of_long_contexts_beside_prompts(gpu, lab):
-    for dim, n in ((64, 20), (128, 5), (64, 70)):
+    for dim, n in ((64, 20), (128, 5), (64, 70), (128, 66)):
         past, counts = [60 * b for b in range(n)], [1] * n
         past[3], counts[1], counts[2], counts[n - 1] = 7000, 150, 0, 40
         check_attention(lab.ops, make_case(n, past, counts, 2, 2, dim, 64, torch.int8))
