@@ -304,6 +304,16 @@ struct Code<true> {
 };
 
 // ------------------------------------------------------------------ append
+//
+// A page's rows of one KV head, all its dimensions, are one scale: the largest
+// magnitude first (a pass over the new rows, kept in registers), then the
+// codes. Keys are stored as they come, values turned (positions of a dimension
+// lie together). Few bytes move (4,096 rows, 8 heads of 64: 13 MB in 6.0 us,
+// 2.1 TB/s, of which launch and slots are 2.6): what bounds it is the chain of
+// slots, rows and, in a page that was begun before, scale and old codes. Of
+// 3,181 rows of 7 requests, 128 dims, 12.4 us, the longest block takes 10.7:
+// it finds five runs that begin in its rows. Runs each to a wave where there
+// are several shorten that (11.8) and lengthen all else by 4 to 10%.
 
 struct Append {
   const uint16_t* x[2];  // keys, values: rows of kv * dim BF16 values
@@ -776,6 +786,16 @@ __device__ __forceinline__ float uniform_of(float v, int lane) {
 // values from the cache straight into the operands' registers, the next
 // unit's while this one is computed (and the page numbers of the one after):
 // no LDS, no barrier until the waves' sums are joined.
+//
+// Where the requests fill the chip, its memory bounds it (64 requests of
+// 3,100 to 4,100 positions, 8 KV heads of 64, int8: 237 MB in 50 us, 4.7
+// TB/s). Below that it is one wave's chain: about 1.7 us a unit, half of it
+// the 192 instructions that make BF16 of int8 codes (FP8: 64), behind 3 us
+// to the first keys (lengths, page numbers, data) and 1.4 for the join. So
+// blocks have eight waves (4 to 8: 64 requests 57 -> 51 us, 8 x 8,192
+// positions of 128 dims 41 -> 31; 16: no better), and few requests are
+// divided into parts of as little as one unit a wave (4,096 positions: 10.9
+// us; two units a wave 12.9).
 template <int D>
 struct NarrowUnit {
   uint4 k[4][D / 64];
@@ -1109,16 +1129,20 @@ __global__ void __launch_bounds__(kWaves* kWave, D == 64 ? 4 : 2) k_kv8_attend_n
 // once for four waves. Groups of four waves share a tile, each with stages of
 // its own and every third (dim 64) or second (128) unit.
 //
-// What bounds it is the vector work around the products (about 290
-// instructions a unit and wave, 80,000 of 160,000 cycles at 3,900 rows x 16
-// heads of 64) and, in what is left, the latency of one wave's chain: one
-// tile's longest chain of units decides how long a chip that holds about two
-// tiles a CU takes. Hence the groups (one group: 77 us, two: 67, three: 67,
-// and 40 -> 38 us for single tokens beside a chunk of 512), the halves of a
-// round (below), and per-segment work moved out of the unit: pages and scales
-// of 64 rounds looked up at once, a lane for each (107 -> 84 us together with
-// 32-bit offsets), nothing per score but the multiply-add, the exponential, a
-// maximum and half a conversion and half a dot product.
+// What bounds it is the vector work around the products (about 280
+// instructions a unit and wave: 74,000 of a SIMD's 150,000 cycles at 3,900
+// rows x 16 heads of 64, the matrix cores busy for 32,000) and, in what is
+// left, the latency of one wave's chain, 2.3 us a round, and 7 us a block for
+// its beginning and its end: one tile's longest chain of units decides how
+// long a chip that holds about two tiles a CU takes. Hence the groups (one
+// group: 77 us, two: 67, three: 67 when that was measured; 61 now), the
+// halves of a round (below), and per-segment work moved out of the unit:
+// pages and scales of 64 rounds looked up at once, a lane for each (107 -> 84
+// us together with 32-bit offsets), nothing per score but the multiply-add,
+// the exponential, half a maximum, half a conversion and half a dot product
+// (a whole maximum: 2% more). Two scores' buffers in turn, two blocks of six
+// waves a CU (80 or 128 registers spill), four groups, and ranges of equal
+// length across the tiles of a batch were no faster.
 constexpr int kWideWaves = 4, kWideColumns = 32 * kWideWaves;
 template <int D>
 struct Wide {
@@ -1608,12 +1632,12 @@ __device__ __forceinline__ void wide_block(const Attend& a, int index, WideShare
   if (!single && half == 0) a.part_ml[part] = float2{all, total};
 }
 
-// Wide tiles first, since they take longest, then the narrow requests. (LDS
-// as dynamic memory: a static array past half of a CU's makes the compiler
-// plan for 512 registers and move results between their two halves.)
-//
-// kItems: narrow items of a block, 0 for a launch without any, 1 where there
-// are few of them (each then has all of the block's waves).
+// Tiles and narrow requests in one launch. kItems: narrow items of a block, 0
+// for a launch without any (one request), 1 where there are few of them (each
+// then has all of the block's waves: 40 rows beside 5 requests on 2,048
+// positions 35.6 -> 21 us). LDS as dynamic memory: a static array past half of
+// a CU's makes the compiler plan for 512 registers and move results between
+// their two halves.
 template <int D, int kItems>
 union BothShared {
   WideShared<D> wide;
@@ -1645,7 +1669,11 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, Wide<D>::kWaves / 4) k_kv8_
 
 // ---- the parts of a split range of keys joined, in the parts' order
 //
-// Four blocks for a request and KV head's narrow columns, or for one wide tile.
+// Four blocks for a request and KV head's narrow columns, or for one wide
+// tile: 4 to 8 us, of which the launch and two dependent loads are most, so
+// the parts' values are asked for before their shares are known (0.3 us) and
+// threads that the columns leave over take parts of their own (63 parts of
+// 15 columns: 11 -> 8 us).
 constexpr int kCombineThreads = 256, kQuarters = 4, kMostShares = 512;  // parts x columns: 64 x 4, 16 x 32
 
 struct CombineShared {

@@ -108,10 +108,13 @@ def attention(q, keys, values, ks, vs, table, past, starts, scale):
     dim exact products in FP32 (each partial sum off by 2 eps of the sum of magnitudes A, an adder that truncates included)
     and four more roundings, so log2(p) is off by (2 dim + 8) eps A log2(e) and p, with the exponential's own 2 eps, by
     r = (2 dim + 8) eps A + 2 eps of itself; numerator and denominator are sums of at most L such terms in FP32 (2 L eps).
-    The numerator's p is rounded to BF16 (2^-8), and so is v scale where the scale is no power of two (2^-8; `exact_scales`
-    has them all powers); the result is rounded to BF16 once more. What falls below FP32's smallest normal number, 2^-126, may
-    become 0: a probability (before the division by their sum, which is 1 or more, since the largest is 1), its product with a
-    value, the result. That is at most 2^-126 (|v| + 1) for each position and 2^-126 once."""
+    p is rounded to BF16, each by its own d with |d| <= 2^-8, in the numerator and in the sum alike, which is off by the mean
+    m = sum p d: (sum p (1 + d) v) / (1 + m) - o = sum p d (v - o) / (1 + m), at most 2^-8 (A_v + |o|) / (1 - 2^-8) with A_v =
+    sum p |v| (the 1.01 has the divisor). The factor that takes a value scale out of the sum again is rounded too (2^-8 |o|,
+    and |o| <= A_v) where it is no power of two (`exact_scales` has them all powers); the result is rounded to BF16 once more.
+    What falls below FP32's smallest normal number, 2^-126, may become 0: a probability (before the division by their sum,
+    which is 1 or more, since the largest is 1), its product with a value, the result. That is at most 2^-126 (|v| + 1) for
+    each position and 2^-126 once."""
     rows, heads, dim = q.shape
     kv, page = keys.shape[1], keys.shape[2]
     group = heads // kv
@@ -138,6 +141,6 @@ def attention(q, keys, values, ks, vs, table, past, starts, scale):
                 rel = (2 * dim + 8) * eps * size.max(1, keepdims=True) + 2 * eps + 2 * length * eps
                 out[r, h * group: (h + 1) * group] = o
                 step = 2.0 ** -8 * (1 if exact_scales else 2)
-                reach[r, h * group: (h + 1) * group] = (step + 2 * rel) * 1.01 * a + 2.0 ** -8 * (np.abs(o) + step * a) + \
-                    2.0 ** -126 * (1 + length * (1 + np.abs(v).max()))
+                reach[r, h * group: (h + 1) * group] = ((step + 2 * rel) * a + 2.0 ** -8 * np.abs(o)) * 1.01 + \
+                    2.0 ** -8 * (np.abs(o) + step * a) + 2.0 ** -126 * (1 + length * (1 + np.abs(v).max()))
     return out, reach
