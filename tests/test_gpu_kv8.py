@@ -553,58 +553,6 @@ def test_serving(gpu, lab, dtype, page, kv, group, dim):
     assert sorted(free + used) == list(range(24))
 
 
-def test_a_captured_pass(gpu, lab):
-    """Plan, append and attention in one graph, replayed as the lengths go on: every replay against the eager calls on a
-    second pool, with other work between."""
-    ops, page, kv, dim, n = lab.ops, 16, 2, 64, 3
-    pools = []
-    for _ in range(2):
-        pools.append(dict(cache=empty_cache(30, kv, page, dim, torch.int8), table=ints(np.full((n, 9), -1)), ring=ints(np.arange(30)),
-                          cursor=ints([0, 30], torch.int64), past=ints(np.zeros(n)), counts=ints([1] * n), starts=ints(np.zeros(n + 1)),
-                          slots=ints(np.zeros(40)), status=ints(np.zeros(n)), qkv=torch.zeros(40, 8 * dim, dtype=torch.bfloat16, device="cuda"),
-                          out=torch.zeros(40, 4, dim, dtype=torch.bfloat16, device="cuda")))
-
-    def one(p):
-        ops.kv8_plan(p["past"], p["counts"], p["table"], p["ring"], p["cursor"], p["starts"], p["slots"], p["cursor"], p["status"], page=page)
-        q, k, v = p["qkv"].split([4 * dim, 2 * dim, 2 * dim], dim=1)
-        ops.kv8_append(k.view(40, kv, dim), v.view(40, kv, dim), p["slots"], *p["cache"])
-        ops.kv8_attention(q.view(40, 4, dim), *p["cache"], p["table"], p["past"], p["starts"], p["out"], max_rows=40)
-
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
-        one(pools[0])
-    g = torch.Generator(device="cuda").manual_seed(1)
-    for counts in ([30, 1, 0], [1, 1, 9], [1, 20, 1], [1, 1, 1], [0, 0, 3], [11, 1, 1]):
-        qkv = torch.randn(40, 8 * dim, generator=g, device="cuda").to(torch.bfloat16)
-        for p in pools:
-            p["qkv"].copy_(qkv), p["counts"].copy_(ints(counts)), p["out"].fill_(7.0)
-        graph.replay()
-        one(pools[1])
-        torch.cuda.synchronize()
-        for name in ("out", "table", "slots", "starts", "cursor", "status", "ring"):
-            assert torch.equal(pools[0][name], pools[1][name]), name
-        for a, b in zip(pools[0]["cache"], pools[1]["cache"]):
-            assert torch.equal(a.view(torch.int8) if a.dtype == torch.int8 else a.nan_to_num(-1), b.view(torch.int8) if b.dtype == torch.int8 else b.nan_to_num(-1))
-        for p in pools:
-            p["past"].add_(p["counts"])
-
-
-def test_two_streams(gpu, lab):
-    """Calls on two streams at once, each with tensors of its own, give what they give alone."""
-    cases = [make_case(s, [2000, 900], [60, 1], 4, 2, 64, 64, torch.int8) for s in (1, 2)]
-    alone = [attend(lab.ops, c) for c in cases]
-    streams = [torch.cuda.Stream() for _ in cases]
-    outs = [torch.full_like(a, 7.0) for a in alone]
-    torch.cuda.synchronize()
-    for _ in range(5):
-        for c, s, o in zip(cases, streams, outs):
-            with torch.cuda.stream(s):
-                attend(lab.ops, c, out=o)
-    torch.cuda.synchronize()
-    for a, o in zip(alone, outs):
-        assert torch.equal(a, o)
-
-
 def test_ops_refuse_gpu_tensors_of_other_shapes(gpu, lab):
     ops = lab.ops
     c = make_case(0, [30], [2], 2, 2, 64, 16, torch.int8)
