@@ -548,7 +548,8 @@ def bf16_f32_matmul(input0, input1, output, *, M: int, K: int, N: int, n_cores: 
 #
 # These calls are short, so their checks are one expression each (a tensor's
 # attribute costs 0.07 us, a call 0.1), and the arguments go over as one packed
-# structure (0.5 us; 24 separate ones take ctypes 2.0): 12.5 -> 7 us a call.
+# structure (0.5 us; 24 separate ones take ctypes 2.0): 12.5 -> 6 us a call,
+# of which 4 are the launch.
 # Where the expression is false, the checks one by one name what is wrong.
 
 KV8_LENGTH, KV8_TABLE, KV8_POOL, KV8_ROWS = 1, 2, 4, 8  # kv8_plan's status
@@ -563,10 +564,13 @@ _APPEND = struct.Struct("@7P2q6i")
 _ATTEND = struct.Struct("@11Pq11if")
 
 
-if hasattr(torch._C, "_cuda_getDevice"):
-    _device = torch._C._cuda_getDevice
-else:  # a torch without this private name
+if hasattr(torch._C, "_cuda_getCurrentRawStream") and hasattr(torch._C, "_cuda_getDevice"):
+    _device, _stream_of = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+else:  # a torch without these private names
     _device = torch.cuda.current_device
+
+    def _stream_of(device: int) -> int:
+        return torch.cuda.current_stream(device).cuda_stream
 
 
 def _here(*tensors) -> None:
@@ -671,7 +675,7 @@ def kv8_plan(past, counts, block_table, free_pages, cursor, row_starts, slots, n
     _lib.call("lfm25_kv8_plan", _PLAN.pack(
         past.data_ptr(), counts.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), cursor.data_ptr(),
         row_starts.data_ptr(), slots.data_ptr(), next_cursor.data_ptr(), status.data_ptr(), n, wide[1], ring, rows, page),
-        _stream())
+        _stream_of(here))
 
 
 def _kv8_append_check(keys, values, slots, key_cache, value_cache, key_scales, value_scales) -> None:
@@ -713,7 +717,7 @@ def kv8_append(keys, values, slots, key_cache, value_cache, key_scales, value_sc
     _lib.call("lfm25_kv8_append", _APPEND.pack(
         keys.data_ptr(), values.data_ptr(), slots.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
         key_scales.data_ptr(), value_scales.data_ptr(), ks[0] if rows > 1 else kv * dim, vs[0] if rows > 1 else kv * dim,
-        rows, pages, page, kv, dim, _KV8_FORMATS[code]), _stream())
+        rows, pages, page, kv, dim, _KV8_FORMATS[code]), _stream_of(here))
 
 
 @functools.lru_cache(maxsize=256)
@@ -792,4 +796,4 @@ def kv8_attention(query, key_cache, value_cache, key_scales, value_scales, block
         block_table.data_ptr(), past.data_ptr(), row_starts.data_ptr(), output.data_ptr(),
         0 if status is None else status.data_ptr(), workspace.data_ptr() if need else 0,
         qs[0] if rows > 1 else heads * dim, table[1], n, rows, heads, max_rows, pages, page, kv, dim,
-        _KV8_FORMATS[code], 0, scale), _stream())
+        _KV8_FORMATS[code], 0, scale), _stream_of(here))
