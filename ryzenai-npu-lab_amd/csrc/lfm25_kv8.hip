@@ -34,7 +34,8 @@ constexpr int kStatusRows = 2;  // attention: row offsets outside the rows, or m
 // and a request's new pages are read from the ring). Not where the cursor is
 // updated in place, which some block may still have to read: then one block,
 // and a second launch for the slots of more rows than kPlanRows (14,459 rows
-// of 1,000 requests: 8.5 + 4.2 us, in blocks 8.7).
+// of 1,000 requests: 8.5 + 4.2 us, in blocks of 512 threads 8.1, of 1,024
+// 8.7, of 256 9.8).
 constexpr int kPlanRows = 8192, kPlanBlocks = 256;
 
 // Inclusive sums over the wave's lanes.
@@ -1936,7 +1937,8 @@ extern "C" int lfm25_kv8_plan(const lfm25_kv8_plan_call* call, lfm25_stream_t st
   };
   if (c.requests <= 64 && c.rows <= 256) plan<64, 1>(c, 1, shift, stream);
   else if (c.requests <= 256 && (c.rows <= 1024 || !in_place)) plan<256, 1>(c, blocks(256), shift, stream);
-  else if (c.requests <= 1024) plan<1024, 1>(c, blocks(1024), shift, stream);
+  else if (c.requests <= 1024 && !in_place) plan<512, 2>(c, blocks(512), shift, stream);
+  else if (c.requests <= 1024) plan<1024, 1>(c, 1, shift, stream);
   else plan<1024, 4>(c, blocks(1024), shift, stream);
   if (c.rows > kPlanRows && in_place)
     hipLaunchKernelGGL(k_kv8_slots, dim3((unsigned)((c.rows + (int64_t)kSlotThreads - 1) / kSlotThreads)), dim3(kSlotThreads), 0, stream,
