@@ -1670,12 +1670,20 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, Wide<D>::kWaves / 4) k_kv8_
 
 // ---- the parts of a split range of keys joined, in the parts' order
 //
-// Four blocks for a request and KV head's narrow columns, or for one wide
-// tile: 4 to 8 us, of which the launch and two dependent loads are most, so
-// the parts' values are asked for before their shares are known (0.3 us) and
-// threads that the columns leave over take parts of their own (63 parts of
-// 15 columns: 11 -> 8 us).
-constexpr int kCombineThreads = 256, kQuarters = 4, kMostShares = 512;  // parts x columns: 64 x 4, 16 x 32
+// Blocks for the columns of a request and KV head, or for a part of a wide
+// tile's, more where there are few of either (a tile's 4 to 8: 64 rows on
+// 8,000 positions 24.6 -> 22.5 us in all, but 22.5 -> 23.4 with 128 tiles;
+// columns of a narrow block 4 to 2: 3 rows on 100,001 positions 34.4 -> 32.5).
+// 4 to 6 us, of which the launch and two dependent loads are most, so the
+// parts' values are asked for before their shares are known (0.3 us) and
+// threads that the columns leave over take parts of their own (63 parts of 15
+// columns: 11 -> 8 us with blocks of four).
+constexpr int kCombineThreads = 256, kMostShares = 512;  // parts x columns: 64 x 4, 16 x 32
+
+struct CombineSplit {
+  int wide_blocks, wide_shift;        // log2 of the blocks of a tile
+  int narrow_shift, narrow_columns;   // of a request and KV head; columns of one
+};
 
 struct CombineShared {
   Found found;
@@ -1704,11 +1712,11 @@ __device__ __forceinline__ void combine_shares(const float2* ml, size_t stride, 
 }
 
 template <int D>
-__global__ void __launch_bounds__(kCombineThreads) k_kv8_combine(const Attend a, int wide_items) {
+__global__ void __launch_bounds__(kCombineThreads) k_kv8_combine(const Attend a, const CombineSplit split) {
   __shared__ CombineShared sh;
-  const int quarter = blockIdx.x % kQuarters, item_at = blockIdx.x / kQuarters;
-  const bool wide = item_at < wide_items;
-  const int index = wide ? item_at : item_at - wide_items, h = index % a.kv;
+  const bool wide = (int)blockIdx.x < split.wide_blocks;
+  const int block = (int)blockIdx.x - (wide ? 0 : split.wide_blocks), shift = wide ? split.wide_shift : split.narrow_shift;
+  const int index = block >> shift, piece = block & ((1 << shift) - 1), h = index % a.kv;
   Request rq;
   int parts, columns, c0 = 0, stride;  // columns of the item, the first of this block's
   size_t from;  // column 0 of part 0
@@ -1729,10 +1737,10 @@ __global__ void __launch_bounds__(kCombineThreads) k_kv8_combine(const Attend a,
     from = ((size_t)part.first * a.kv + h) * 16;
     stride = 16 * a.kv;
   }
-  const int mine = wide ? kWideColumns / kQuarters : 16 / kQuarters;
-  from += quarter * mine;
-  columns = min(columns - quarter * mine, mine);
-  c0 += quarter * mine;
+  const int mine = wide ? kWideColumns >> shift : split.narrow_columns;
+  from += piece * mine;
+  columns = min(columns - piece * mine, mine);
+  c0 += piece * mine;
   if (columns <= 0) return;
   // Where the columns leave threads over, those take a share of the parts
   // each, so that a part's load does not wait for the one eight before it. The
@@ -1901,10 +1909,20 @@ int attend(const Attend& a, const Splits& s, hipStream_t stream) {
     attend_narrow<D, kFp8, 8>(a, narrow, stream);
   }
   if (s.share > 0 || (s.has_wide && s.wide > 1)) {
-    // (a tile in parts is one of at most kWideParts / 2)
-    const int wide_items = s.has_wide && s.wide > 1 ? kWideParts / 2 : 0;
-    const int64_t narrow_items = s.share > 0 ? (int64_t)a.requests * a.kv : 0;
-    hipLaunchKernelGGL((k_kv8_combine<D>), dim3((unsigned)((wide_items + narrow_items) * kQuarters)), dim3(kCombineThreads), 0, stream, a, wide_items);
+    CombineSplit c{};
+    if (s.has_wide && s.wide > 1) {  // (a tile in parts is one of at most kWideParts / 2)
+      const int items = (int)std::min<int64_t>(kWideParts / 2, s.wide_tiles * a.kv);
+      c.wide_shift = items <= 64 ? 3 : 2;
+      c.wide_blocks = items << c.wide_shift;
+    }
+    int narrow_blocks = 0;
+    if (s.share > 0) {
+      const int64_t columns = std::min<int64_t>(16, (int64_t)a.max_rows * a.group), items = (int64_t)a.requests * a.kv;
+      c.narrow_columns = columns > 4 && items * columns <= 512 ? 2 : 4;
+      while ((c.narrow_columns << c.narrow_shift) < columns) ++c.narrow_shift;
+      narrow_blocks = (int)(items << c.narrow_shift);
+    }
+    hipLaunchKernelGGL((k_kv8_combine<D>), dim3((unsigned)(c.wide_blocks + narrow_blocks)), dim3(kCombineThreads), 0, stream, a, c);
   }
   return check_launch("lfm25_kv8_attention");
 }
