@@ -12,7 +12,6 @@ int8 or float8_e4m3fn, FP32 scales [pages, kv_heads] for each of the two
 of page numbers. Rows of a pass are packed request after request.
 """
 
-import functools
 import importlib
 import math
 import random
@@ -231,14 +230,9 @@ def prepare(case, seed):
 
 # ---------------------------------------------------------------- one pass
 
-@functools.lru_cache(1)
-def _framework():
-    return importlib.import_module("ryzenai-npu-lab_amd").ops
-
-
 def run(s):
     if own:
-        ops = _framework()
+        ops = importlib.import_module("ryzenai-npu-lab_amd").ops
         if s["op"] == "plan":
             ops.kv8_plan(s["past"], s["counts"], s["block_table"], s["free_pages"], s["cursor"], s["row_starts"], s["slots"],
                          s["next_cursor"], s["status"], page=s["page"])
