@@ -605,8 +605,8 @@ __global__ void __launch_bounds__(kAppendThreads, 6) k_kv8_append(const Append a
 // Neither costs an operation per score: the key scale is the factor of the
 // exponent's one fused multiply-add, the value scale (less the largest seen,
 // so that no sum passes the range of the values) its addend as a logarithm,
-// and the sum of the probabilities takes that factor back out as the other
-// operand of its dot product.
+// and the sum of a segment's probabilities takes that factor back out in FP32,
+// one operation a segment.
 constexpr int kUnit = 64;
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -748,16 +748,14 @@ __device__ __forceinline__ Scales scales_of(const Attend& a, size_t head, bool b
 }
 
 // The logarithm of a segment's value scale against the largest so far (0 for
-// one whose values count as 0), and the pair of factors that takes it out of
-// the sum again. Not below 2^-64: values that small beside the largest are
-// far below its rounding, and the factors stay numbers.
+// one whose values count as 0). Not below 2^-64: values that small beside the
+// largest are far below its rounding, and the factor that takes it out of the
+// sum again stays a number. (That factor is FP32: rounded to BF16 it would put
+// a whole page's share of the sum off by up to 2^-8.)
 __device__ __forceinline__ float relative(float lv, float top) { return lv == -INFINITY ? 0.0f : fmaxf(lv - top, -64.0f); }
-__device__ __forceinline__ uint32_t undo(float d) {
-  const float w = exp2_of(-d);
-  return pack_bf16(w, w);
-}
-__device__ __forceinline__ float dot2(uint32_t p, uint32_t w, float sum) {
-  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p), __builtin_bit_cast(bf16x2, w), sum, false);
+// The sum of two BF16 numbers and an FP32 one.
+__device__ __forceinline__ float add2(uint32_t p, float sum) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p), __builtin_bit_cast(bf16x2, 0x3f803f80u), sum, false);
 }
 
 // The running statistics of a column (a query): the maximum m that its
@@ -1050,7 +1048,7 @@ __device__ __forceinline__ void narrow_block(const Attend& a, int index, int w, 
       top = new_top;
     }
     const float d = relative(sc.lv, top), add = d - (m == -INFINITY ? 0.0f : m);
-    const uint32_t back = undo(d);
+    float part = 0.0f;  // the segment's probabilities times 2^d
     // The probabilities are rounded to BF16, the value product's operand
     // type: up to 2^-8 of each, the same rounded ones in the sum.
     bf16x8 p[2];
@@ -1067,11 +1065,12 @@ __device__ __forceinline__ void narrow_block(const Attend& a, int index, int w, 
         }
         pk[2 * t] = pack_bf16(e[0], e[1]);
         pk[2 * t + 1] = pack_bf16(e[2], e[3]);
-        sum = dot2(pk[2 * t], back, sum);
-        sum = dot2(pk[2 * t + 1], back, sum);
+        part = add2(pk[2 * t], part);
+        part = add2(pk[2 * t + 1], part);
       }
       p[c] = __builtin_bit_cast(bf16x8, uint4{pk[0], pk[1], pk[2], pk[3]});
     }
+    sum = fmaf(part, exp2_of(-d), sum);
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) {
       o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes8<kFp8>(x.v[t].x, x.v[t].y), p[0], o[t], 0, 0, 0);
@@ -1337,19 +1336,18 @@ __device__ __forceinline__ void wide_unit(const WideStages<D>& sh, int first, in
     x.top = new_top;
   }
   const float against = x.m == -INFINITY ? 0.0f : x.m;
-  float add[4];
-  uint32_t back[4];
+  float add[4], back[4];
   {
     const float d = relative(sc[0].lv, x.top);
     add[0] = add[1] = add[2] = add[3] = d - against;
-    back[0] = back[1] = back[2] = back[3] = undo(d);
+    back[0] = back[1] = back[2] = back[3] = exp2_of(-d);
   }
   if (!one_page) {
 #pragma unroll
     for (int i = 1; i < 4; ++i) {
       const float d = relative(sc[i].lv, x.top);
       add[i] = d - against;
-      back[i] = undo(d);
+      back[i] = exp2_of(-d);
     }
   }
 #pragma unroll
@@ -1364,10 +1362,7 @@ __device__ __forceinline__ void wide_unit(const WideStages<D>& sh, int first, in
       }
       // (rounded to BF16 as in the narrow form)
       const uint4 pk{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])};
-      x.sum = dot2(pk.x, back[2 * t + e], x.sum);
-      x.sum = dot2(pk.y, back[2 * t + e], x.sum);
-      x.sum = dot2(pk.z, back[2 * t + e], x.sum);
-      x.sum = dot2(pk.w, back[2 * t + e], x.sum);
+      x.sum = fmaf(add2(pk.w, add2(pk.z, add2(pk.y, add2(pk.x, 0.0f)))), back[2 * t + e], x.sum);
       const bf16x8 p = __builtin_bit_cast(bf16x8, pk);
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
