@@ -653,11 +653,11 @@ int lfm25_kv8_append(const lfm25_kv8_append_call* c, lfm25_stream_t stream);
  * softmax(scale * q . k). query: BF16 rows [heads x head_dim] at query + r *
  * query_stride (elements, a multiple of 8); output [rows x heads x head_dim]
  * BF16, contiguous; heads = kv_heads * group, group in [1, 16], query head j
- * with KV head j / group. FP32 scores, sums and statistics; probabilities are
- * rounded to BF16 for the value product, and a value scale below 2^-64 of the
- * largest among the positions that count counts as that. max_rows: no request
- * brings more rows. A row that sees no position (past[b] + i < 0) is
- * zero; rows behind row_starts[requests] are left as they were. status (int32,
+ * with KV head j / group. FP32 scores, sums and statistics; the products of
+ * probability and value scale are rounded to BF16 for the value product (2^-8
+ * of each), and what of them is below 2^-126 of the largest may count as 0.
+ * max_rows: no request brings more rows. A row that sees no position (past[b]
+ * + i < 0) is zero; rows behind row_starts[requests] are left as they were. status (int32,
  * may be NULL), set and never cleared here: bit 0, a page number outside the
  * pool or a position past the table: rows that attend to it are NaN; bit 1,
  * a request with row offsets outside the rows or out of order, or with more

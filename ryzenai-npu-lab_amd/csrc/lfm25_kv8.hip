@@ -603,8 +603,7 @@ __global__ void __launch_bounds__(kAppendThreads, 6) k_kv8_append(const Append a
 // A unit is 64 positions: four segments of 16, each within one page (pages
 // are multiples of 16 positions), so a segment has one key and value scale.
 // Neither costs an operation per score: the key scale is the factor of the
-// exponent's one fused multiply-add, the value scale (less the largest seen,
-// so that no sum passes the range of the values) its addend as a logarithm,
+// exponent's one fused multiply-add, the value scale its addend as a logarithm,
 // and the sum of a segment's probabilities takes that factor back out in FP32,
 // one operation a segment.
 constexpr int kUnit = 64;
@@ -723,11 +722,13 @@ __device__ __forceinline__ float largest(float a, float b, float c) {
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float nan_of() { return __uint_as_float(0x7fc00000u); }
 
-// log2 of a value scale, whole for a power of two; -inf for one without
-// effect (0, a subnormal), NaN for one that is not finite or is negative.
+// log2 of a value scale, whole for a power of two; kNoValue for one without
+// effect (0, a subnormal; below any other's, and a number, so that nothing below
+// has to tell it from them), NaN for one that is not finite or is negative.
+constexpr float kNoValue = -150.0f;
 __device__ __forceinline__ float scale_log2(float s) {
   const uint32_t u = __float_as_uint(s);
-  if ((u & 0x7f800000u) == 0u) return -INFINITY;
+  if ((u & 0x7f800000u) == 0u) return kNoValue;
   if (u >= 0x7f800000u) return nan_of();
   const uint32_t m = u & 0x7fffffu;
   return (float)((int)(u >> 23) - 127) + (m ? __builtin_amdgcn_logf(__uint_as_float(0x3f800000u | m)) : 0.0f);
@@ -739,39 +740,48 @@ __device__ __forceinline__ float scale_log2(float s) {
 // scores are replaced, and its values count as 0.
 struct Scales {
   float ks;  // key scale * log2(e) * softmax scale
-  float lv;  // log2 of the value scale; -inf: the values count as 0
+  float lv;  // log2 of the value scale; kNoValue: the values count as 0
 };
 __device__ __forceinline__ Scales scales_of(const Attend& a, size_t head, bool bad) {
   Scales s{a.ks[head] * a.scale, scale_log2(a.vs[head])};
-  if (bad || s.lv != s.lv) s = Scales{nan_of(), -INFINITY};
+  if (bad || s.lv != s.lv) s = Scales{nan_of(), kNoValue};
   return s;
 }
 
-// The logarithm of a segment's value scale against the largest so far (0 for
-// one whose values count as 0). Not below 2^-64: values that small beside the
-// largest are far below its rounding, and the factor that takes it out of the
-// sum again stays a number. (That factor is FP32: rounded to BF16 it would put
-// a whole page's share of the sum off by up to 2^-8.)
-__device__ __forceinline__ float relative(float lv, float top) { return lv == -INFINITY ? 0.0f : fmaxf(lv - top, -64.0f); }
 // The sum of two BF16 numbers and an FP32 one.
 __device__ __forceinline__ float add2(uint32_t p, float sum) {
   return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p), __builtin_bit_cast(bf16x2, 0x3f803f80u), sum, false);
 }
 
-// The running statistics of a column (a query): the maximum m that its
-// exponents are against, the sum, and the largest value scale `top` (of the
-// whole wave). They move only when a score passes m by more than 2^8, or the
-// scales grow: an m below the maximum leaves every p below 2^8 and their
-// ratios as they are.
-constexpr float kSlack = 8.0f;
+// The running statistics of a column (a query), all its own. With t a score
+// and lv the log2 of its position's value scale: m is the largest t and `top`
+// the largest t + lv that it sees (kLowest, a number, before it sees any). The
+// value product's weights are e = 2^(t + lv - top), so that none is above 1 and
+// the largest is 1, whatever the scales; the probabilities of the sum are 2^(t
+// - m) = e 2^(top - m - lv), one factor for a segment's.
+//
+// Where that factor is past 2^64 (a page whose scale is that far below what
+// the others make of the row; 2^-120 is that of a page of zeros) the weights
+// would lose what the sum needs: then it takes exponentials of its own.
+//
+// Both maxima move only when they are passed by more than 2^8: that leaves
+// every weight below 2^8 and their ratios as they are.
+constexpr float kLowest = -0x1.fffffep127f, kSlack = 8.0f, kMostBack = 64.0f;
+
+// 2^(top - m) as two factors, since it may be smaller than FP32's smallest normal number.
+struct Unit {
+  float a, b;
+};
+__device__ __forceinline__ Unit unit_of(float top, float m) {
+  const float x = fmaxf(top - m, -400.0f), h = __builtin_rintf(0.5f * x);  // (whole, if x is)
+  return Unit{exp2_of(h), exp2_of(x - h)};
+}
 
 constexpr int kMostNarrowParts = 64;  // of one request
 
-// A part's share of a whole: its sum against the common maximum, 0 for a part
-// that saw nothing (m = -inf).
-__device__ __forceinline__ float part_weight(float m, float all, float sum) {
-  return (m == -INFINITY ? 0.0f : exp2_of(m - all)) * sum;
-}
+// A part's share of a whole: its sum against the common maximum (0 for a part
+// that saw nothing).
+__device__ __forceinline__ float part_weight(float m, float all, float sum) { return exp2_of(m - all) * sum; }
 
 __device__ __forceinline__ int uniform_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 __device__ __forceinline__ float uniform_of(float v, int lane) {
@@ -988,7 +998,7 @@ __device__ __forceinline__ void narrow_block(const Attend& a, int index, int w, 
       q[c] = __builtin_bit_cast(bf16x8, x);
     }
   }
-  float m = -INFINITY, sum = 0.0f, top = -INFINITY;
+  float m = kLowest, top = kLowest, sum = 0.0f;
   f32x4 o[D / 16];
 #pragma unroll
   for (int t = 0; t < D / 16; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -1010,9 +1020,9 @@ __device__ __forceinline__ void narrow_block(const Attend& a, int index, int w, 
     const bool inside = at < rq.len;
     Scales sc{x.ks * a.scale, scale_log2(x.vs)};
     if (x.bad) raise(a.status, kStatusPage);
-    const bool none = x.bad || !(sc.lv > -INFINITY);  // the segment's values count as 0
-    if (x.bad || sc.lv != sc.lv) sc.ks = nan_of();
-    if (none || !inside) sc.lv = -INFINITY;
+    if (x.bad || sc.lv != sc.lv) sc = Scales{nan_of(), kNoValue};
+    const bool none = sc.lv == kNoValue;  // the segment's values count as 0
+    if (!inside) sc.lv = 0.0f;
     const bool whole = u * kUnit + kUnit - 1 <= rq.past && __ballot(none) == 0;  // seen by every column
     if (!whole) {
       // values behind the last position may be anything
@@ -1036,21 +1046,34 @@ __device__ __forceinline__ void narrow_block(const Attend& a, int index, int w, 
 #pragma unroll
     for (int t = 0; t < 4; ++t) most = largest(most, s[t][0], largest(s[t][1], s[t][2], s[t][3]));
     // (a segment that the column sees nothing of has -inf here, whatever its scale)
-    most = across_max16(most == -INFINITY ? most : most * sc.ks);
-    const float new_top = fmaxf(top, across_max16(sc.lv));
-    if (__ballot(most > m + kSlack || new_top > top) != 0) {
-      const float m_new = fmaxf(m, most), to = m_new == -INFINITY ? 0.0f : m_new;
-      const float shrink = exp2_of(m - to), shrink_top = exp2_of(top == -INFINITY ? 0.0f : top - new_top);
-      sum *= shrink;
+    most = most == -INFINITY ? most : most * sc.ks;
+    const float most_top = across_max16(most + sc.lv);
+    most = across_max16(most);
+    bool far = false;  // the sum has taken exponentials of its own
+    if (__ballot(most > m + kSlack || most_top > top + kSlack || top - m - sc.lv > kMostBack) != 0) {
+      const float m_new = fmaxf(m, most), top_new = fmaxf(top, most_top);
+      const float shrink = exp2_of(top - top_new);
+      sum *= exp2_of(m - m_new);
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t) o[t] *= shrink * shrink_top;
+      for (int t = 0; t < D / 16; ++t) o[t] *= shrink;
       m = m_new;
-      top = new_top;
+      top = top_new;
+      far = __ballot(top - m - sc.lv > kMostBack) != 0;
+      if (far) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e = exp2_of(fmaf(s[t][i], sc.ks, -m));
+            sum += !whole && at + 4 * t + i > pos ? 0.0f : e;
+          }
+      }
     }
-    const float d = relative(sc.lv, top), add = d - (m == -INFINITY ? 0.0f : m);
-    float part = 0.0f;  // the segment's probabilities times 2^d
-    // The probabilities are rounded to BF16, the value product's operand
-    // type: up to 2^-8 of each, the same rounded ones in the sum.
+    const float add = sc.lv - top;
+    float part = 0.0f;  // the sum of the segment's weights
+    // The weights are rounded to BF16, the value product's operand type: up to
+    // 2^-8 of each, the same rounded ones in the sum. (FP16 has the bits but
+    // not the range: beside a weight of 1 whose value is 0, 2^-50 still counts.)
     bf16x8 p[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -1070,7 +1093,7 @@ __device__ __forceinline__ void narrow_block(const Attend& a, int index, int w, 
       }
       p[c] = __builtin_bit_cast(bf16x8, uint4{pk[0], pk[1], pk[2], pk[3]});
     }
-    sum = fmaf(part, exp2_of(-d), sum);
+    if (!far) sum = fmaf(part, exp2_of(top - m - sc.lv), sum);
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) {
       o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes8<kFp8>(x.v[t].x, x.v[t].y), p[0], o[t], 0, 0, 0);
@@ -1080,14 +1103,15 @@ __device__ __forceinline__ void narrow_block(const Attend& a, int index, int w, 
   // Join the waves, each as its own result (so that nothing passes the range
   // of the values): o of this lane is column r, dimensions 16 t + 4 g + i.
   sum = across_sum16(sum);
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, unit = exp2_of(top);
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const Unit unit = unit_of(top, m);
   if (g == 0) {
     sh.m[w][r] = m;
     sh.l[w][r] = sum;
   }
 #pragma unroll
   for (int t = 0; t < D / 16; ++t)
-    *reinterpret_cast<f32x4*>(&sh.o[w][r][16 * t + 4 * g]) = o[t] * inv * unit;
+    *reinterpret_cast<f32x4*>(&sh.o[w][r][16 * t + 4 * g]) = o[t] * inv * unit.a * unit.b;
   __syncthreads();
   const int heads = a.kv * a.group;
   for (int e = w * kWave + l; e < columns * (D / 4); e += kWaves * kWave) {
@@ -1209,8 +1233,8 @@ __device__ __forceinline__ WideTable wide_table(const Attend& a, const WideEntry
   WideTable x;
   x.id = e.id;
   x.s = Scales{e.ks * a.scale, scale_log2(e.vs)};
-  if (!e.inside) x.s = Scales{0.0f, -INFINITY};
-  else if (e.bad || x.s.lv != x.s.lv) x.s = Scales{nan_of(), -INFINITY};
+  if (!e.inside) x.s = Scales{0.0f, 0.0f};  // (seen by no column)
+  else if (e.bad || x.s.lv != x.s.lv) x.s = Scales{nan_of(), kNoValue};
   return x;
 }
 
@@ -1246,10 +1270,10 @@ __device__ __forceinline__ void store_values(WideStages<D>& sh, int w, int end, 
   const int l = lane_id();
   sh.s[w] = x.of_v.s;  // (every lane the same)
   const int left = end - x.of_v.at;
-  if (left < 16 || x.of_v.s.lv == -INFINITY) {
+  if (left < 16 || x.of_v.s.lv == kNoValue) {
     // What lies behind the last position may be anything, and the values of
     // a page or scale that is no number count as 0.
-    const int keep = x.of_v.s.lv == -INFINITY ? 0 : left;
+    const int keep = x.of_v.s.lv == kNoValue ? 0 : left;
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) {
       uint32_t* const v = reinterpret_cast<uint32_t*>(&x.v[c]);
@@ -1273,7 +1297,8 @@ template <int D>
 struct WideState {
   bf16x8 q[D / 16];
   f32x16 o[D / 32];
-  float m, sum, top;
+  float m, top, sum;
+  float m_past, top_past, top_m;  // m + kSlack, top + kSlack, top - m
 };
 struct WideScores {
   f32x16 t[2];  // positions 32 t ..
@@ -1314,41 +1339,57 @@ __device__ __forceinline__ void wide_unit(const WideStages<D>& sh, int first, in
       for (int i = 0; i < 16; ++i)
         if (32 * t + 16 * (i / 8) + i % 8 > behind) s.t[t][i] = -INFINITY;
   }
-  float most = -INFINITY;
+  float each[4];  // the segments' largest
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const auto at = [&](int i) { return s.t[t][8 * e + i]; };
-      const float v = largest(largest(at(0), at(1), at(2)), largest(at(3), at(4), at(5)), __builtin_elementwise_maximum(at(6), at(7)));
-      // (where the column sees nothing of the segment: -inf, whatever its scale)
-      most = fmaxf(most, kMasked && v == -INFINITY ? v : v * sc[2 * t + e].ks);
-    }
-  most = across_max32(most);
-  const float new_top = fmaxf(fmaxf(x.top, fmaxf(sc[0].lv, sc[1].lv)), fmaxf(sc[2].lv, sc[3].lv));
-  if (__ballot(most > x.m + kSlack || new_top > x.top) != 0) {
-    const float m_new = fmaxf(x.m, most), to = m_new == -INFINITY ? 0.0f : m_new;
-    const float shrink = exp2_of(x.m - to), shrink_top = exp2_of(x.top == -INFINITY ? 0.0f : x.top - new_top);
-    x.sum *= shrink;
-#pragma unroll
-    for (int t = 0; t < D / 32; ++t) x.o[t] *= shrink * shrink_top;
-    x.m = m_new;
-    x.top = new_top;
+  for (int i = 0; i < 4; ++i) {
+    const auto at = [&](int k) { return s.t[i / 2][8 * (i % 2) + k]; };
+    each[i] = largest(largest(at(0), at(1), at(2)), largest(at(3), at(4), at(5)), __builtin_elementwise_maximum(at(6), at(7)));
   }
-  const float against = x.m == -INFINITY ? 0.0f : x.m;
+  // (what the column sees nothing of is -inf, whatever its scale)
+  const auto scaled = [&](float v, float ks) { return kMasked && v == -INFINITY ? v : v * ks; };
+  float most, most_top, least;
+  if (one_page) {
+    most = across_max32(scaled(fmaxf(fmaxf(each[0], each[1]), fmaxf(each[2], each[3])), sc[0].ks));
+    most_top = most + sc[0].lv;
+    least = sc[0].lv;
+  } else {
+    float top[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      each[i] = scaled(each[i], sc[i].ks);
+      top[i] = each[i] + sc[i].lv;
+    }
+    most = across_max32(fmaxf(fmaxf(each[0], each[1]), fmaxf(each[2], each[3])));
+    most_top = across_max32(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+    least = fminf(fminf(sc[0].lv, sc[1].lv), fminf(sc[2].lv, sc[3].lv));
+  }
+  bool far = false;  // the sum has taken exponentials of its own
+  if (__ballot(most > x.m_past || most_top > x.top_past || x.top_m - least > kMostBack) != 0) {
+    const float m_new = fmaxf(x.m, most), top_new = fmaxf(x.top, most_top);
+    const float shrink = exp2_of(x.top - top_new);
+    x.sum *= exp2_of(x.m - m_new);
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) x.o[t] *= shrink;
+    x.m = m_new, x.m_past = m_new + kSlack;
+    x.top = top_new, x.top_past = top_new + kSlack;
+    x.top_m = top_new - m_new;
+    far = __ballot(x.top_m - least > kMostBack) != 0;
+    if (far) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float f = exp2_of(fmaf(s.t[t][i], sc[2 * t + i / 8].ks, -x.m));
+          x.sum += kMasked && 32 * t + 16 * (i / 8) + i % 8 > behind ? 0.0f : f;
+        }
+    }
+  }
+  const float of = far ? kLowest : x.top_m;  // (every factor 0)
   float add[4], back[4];
-  {
-    const float d = relative(sc[0].lv, x.top);
-    add[0] = add[1] = add[2] = add[3] = d - against;
-    back[0] = back[1] = back[2] = back[3] = exp2_of(-d);
-  }
-  if (!one_page) {
 #pragma unroll
-    for (int i = 1; i < 4; ++i) {
-      const float d = relative(sc[i].lv, x.top);
-      add[i] = d - against;
-      back[i] = exp2_of(-d);
-    }
+  for (int i = 0; i < 4; ++i) {
+    add[i] = sc[i].lv - x.top;
+    back[i] = exp2_of(of - sc[i].lv);
   }
 #pragma unroll
   for (int t = 0; t < 2; ++t)
@@ -1530,7 +1571,8 @@ __device__ __forceinline__ void wide_block(const Attend& a, int index, WideShare
       x.q[c] = __builtin_bit_cast(bf16x8, y);
     }
   }
-  x.m = x.top = -INFINITY;
+  x.m = x.top = x.m_past = x.top_past = kLowest;
+  x.top_m = 0.0f;
   x.sum = 0.0f;
 #pragma unroll
   for (int t = 0; t < D / 32; ++t) x.o[t] = f32x16{};
@@ -1585,14 +1627,15 @@ __device__ __forceinline__ void wide_block(const Attend& a, int index, WideShare
   if (!(group & 1)) lds_barrier();
   // join the groups, each as its own result
   x.sum = across_sum32(x.sum);
-  const float inv = x.sum == 0.0f ? 0.0f : 1.0f / x.sum, unit = exp2_of(x.top);
+  const float inv = x.sum == 0.0f ? 0.0f : 1.0f / x.sum;
+  const Unit unit = unit_of(x.top, x.m);
   const int c = 32 * w4 + (l & 31);
   if (group) {
 #pragma unroll
     for (int t = 0; t < D / 32; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        sh.o[group - 1][c][8 * t + 2 * i + half] = f32x4{x.o[t][4 * i], x.o[t][4 * i + 1], x.o[t][4 * i + 2], x.o[t][4 * i + 3]} * inv * unit;
+        sh.o[group - 1][c][8 * t + 2 * i + half] = f32x4{x.o[t][4 * i], x.o[t][4 * i + 1], x.o[t][4 * i + 2], x.o[t][4 * i + 3]} * inv * unit.a * unit.b;
     if (half == 0) sh.ml[group - 1][c] = float2{x.m, x.sum};
   }
   __syncthreads();
@@ -1614,7 +1657,7 @@ __device__ __forceinline__ void wide_block(const Attend& a, int index, WideShare
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int d = 32 * t + 8 * i + 4 * half;
-      f32x4 y = f32x4{x.o[t][4 * i], x.o[t][4 * i + 1], x.o[t][4 * i + 2], x.o[t][4 * i + 3]} * (share[0] * inv) * unit;
+      f32x4 y = f32x4{x.o[t][4 * i], x.o[t][4 * i + 1], x.o[t][4 * i + 2], x.o[t][4 * i + 3]} * (share[0] * inv) * unit.a * unit.b;
 #pragma unroll
       for (int g = 1; g < kGroups; ++g) y += sh.o[g - 1][c][8 * t + 2 * i + half] * share[g];
       if (single) {
