@@ -722,16 +722,14 @@ __device__ __forceinline__ float largest(float a, float b, float c) {
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float nan_of() { return __uint_as_float(0x7fc00000u); }
 
-// log2 of a value scale, whole for a power of two; kNoValue for one without
-// effect (0, a subnormal; below any other's, and a number, so that nothing below
-// has to tell it from them), NaN for one that is not finite or is negative.
+// log2 of a value scale, whole for a power of two; kNoValue for 0 (below any
+// scale's, subnormal ones included, and a number, so that nothing below has to
+// tell it from the others), NaN for one that is not finite or is negative.
 constexpr float kNoValue = -150.0f;
 __device__ __forceinline__ float scale_log2(float s) {
-  const uint32_t u = __float_as_uint(s);
-  if ((u & 0x7f800000u) == 0u) return kNoValue;
-  if (u >= 0x7f800000u) return nan_of();
-  const uint32_t m = u & 0x7fffffu;
-  return (float)((int)(u >> 23) - 127) + (m ? __builtin_amdgcn_logf(__uint_as_float(0x3f800000u | m)) : 0.0f);
+  if (__float_as_uint(s) > 0x7f7fffffu) return s == 0.0f ? kNoValue : nan_of();
+  const float m = __builtin_amdgcn_frexp_mantf(s);  // in [1/2, 1), of subnormals too; 0 for 0
+  return fmaxf((float)__builtin_amdgcn_frexp_expf(s) + (m == 0.5f ? -1.0f : __builtin_amdgcn_logf(m)), kNoValue);
 }
 
 // A segment's scales as the kernels use them. A page that cannot be read, or
