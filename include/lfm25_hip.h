@@ -574,8 +574,10 @@ int lfm25_batch_linear(const uint16_t* x, const uint16_t* w, uint16_t* y, int32_
  * of its positions; entries past what it holds may be anything. A pass brings
  * rows, packed request after request: request b's are rows row_starts[b] ..
  * row_starts[b + 1), at positions past[b], past[b] + 1, ... A page may be in
- * several tables (a shared beginning), but rows may be appended to it for one
- * request only. The three calls of a pass, in order on one stream, are
+ * several requests' rows of the table (a shared beginning), but is one
+ * request's own: rows are appended to it for that one only, and
+ * lfm25_kv8_plan_with() is told which pages are not the others' own. The three
+ * calls of a pass, in order on one stream, are
  * lfm25_kv8_plan, lfm25_kv8_append (for each layer's pool; the page numbers
  * are the same) and lfm25_kv8_attention; all may be captured into a graph,
  * whose replays read the lengths of the moment. */
@@ -584,7 +586,7 @@ int lfm25_batch_linear(const uint16_t* x, const uint16_t* w, uint16_t* y, int32_
 #define LFM25_KV8_MAX_REQUESTS 4096
 
 /* Why lfm25_kv8_plan refused a request (status[b]; 0: it did not). */
-#define LFM25_KV8_LENGTH 1 /* past[b] is negative, or more than the table's row holds */
+#define LFM25_KV8_LENGTH 1 /* past[b] is negative, more than the table's row holds, or among shared pages */
 #define LFM25_KV8_TABLE 2  /* the new rows go past the table's row */
 #define LFM25_KV8_POOL 4   /* no free pages for the new rows, or (an ending request) no room in the ring */
 #define LFM25_KV8_ROWS 8   /* the new rows go past `rows` */
@@ -597,8 +599,8 @@ int lfm25_batch_linear(const uint16_t* x, const uint16_t* w, uint16_t* y, int32_
  *
  * Each request in order takes the pages that its new rows need from the ring
  * (they go to its block_table row behind those it holds), or, ending, gives
- * its pages back (behind cursor[1]; they are free from the next call on, and
- * its table row is left as it is). row_starts: int32 [requests + 1], the sum
+ * every page that it holds back (behind cursor[1]; they are free from the next
+ * call on, and its table row is left as it is). row_starts: int32 [requests + 1], the sum
  * of the counts before each request (those of refused ones too: its rows are
  * in the pass). slots: int32 [rows], page * page size + position within it of
  * each row; -1 for a refused request's rows and for those behind the last.
@@ -620,6 +622,18 @@ typedef struct lfm25_kv8_plan_call {
   int32_t requests, width, ring, rows, page;
 } lfm25_kv8_plan_call;
 int lfm25_kv8_plan(const lfm25_kv8_plan_call* c, lfm25_stream_t stream);
+
+/* lfm25_kv8_plan() for tables that share pages. shared (int32 [requests]; NULL:
+ * as if all 0): the first shared[b] pages of request b's row are not its own.
+ * Ending, it keeps them out of the ring; new rows have to begin behind them
+ * (otherwise, and where shared[b] is outside [0, width]: LFM25_KV8_LENGTH).
+ * Each page is then given back once, when the request ends whose own it is:
+ * let that one end after the others that have the page (until then it may
+ * rest, with counts[b] = 0). */
+typedef struct lfm25_kv8_plan_pages {
+  const int32_t* shared;
+} lfm25_kv8_plan_pages;
+int lfm25_kv8_plan_with(const lfm25_kv8_plan_call* c, const lfm25_kv8_plan_pages* pages, lfm25_stream_t stream);
 
 /* New keys and values into the cache: row r ([kv_heads x head_dim] BF16 at
  * keys + r * key_stride, in elements, a multiple of 8; values alike) goes to

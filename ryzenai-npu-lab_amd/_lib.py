@@ -130,6 +130,7 @@ SIGNATURES = {
     "lfm25_batch_linear": (ctypes.c_int, [_p, _p, _p, _i32, _i32, _i32, _p]),
     # (the kv8 calls' structures are packed by ops.py, as bytes)
     "lfm25_kv8_plan": (ctypes.c_int, [ctypes.c_char_p, _p]),
+    "lfm25_kv8_plan_with": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, _p]),
     "lfm25_kv8_append": (ctypes.c_int, [ctypes.c_char_p, _p]),
     "lfm25_kv8_attention_workspace_bytes": (_size, [_i32] * 8),
     "lfm25_kv8_attention": (ctypes.c_int, [ctypes.c_char_p, _p]),

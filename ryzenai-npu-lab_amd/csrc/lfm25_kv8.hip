@@ -98,22 +98,25 @@ __device__ __forceinline__ int block_sums(int v, int* waves, int& total) {
   return __builtin_elementwise_add_sat(before, below);
 }
 
-// kThreads threads, requests up to kEach a thread.
+// kThreads threads, requests up to kEach a thread. `shared`: pages at each
+// request's beginning that are not its own (null: none).
 template <int kThreads, int kEach>
 __global__ void __launch_bounds__(kThreads) k_kv8_plan(const int* __restrict__ past, const int* __restrict__ counts, int n,
                                                        int* table, int width, int* ring, int ring_n, const int64_t* cursor,
                                                        int* __restrict__ row_starts, int* __restrict__ slots, int rows,
-                                                       int64_t* next_cursor, int* __restrict__ status, int shift) {
+                                                       int64_t* next_cursor, int* __restrict__ status, int shift,
+                                                       const int* __restrict__ shared) {
   extern __shared__ uint4 dynamic[];
   PlanShared<kThreads * kEach>& sh = *reinterpret_cast<PlanShared<kThreads * kEach>*>(dynamic);
   const int t = threadIdx.x, page = 1 << shift, everyone = (int)gridDim.x * kThreads, me = (int)blockIdx.x * kThreads + t;
   const bool first_block = blockIdx.x == 0;
-  int p[kEach], c[kEach];
+  int p[kEach], c[kEach], others[kEach];
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
     const int b = t * kEach + j;
     p[j] = b < n ? past[b] : 0;
     c[j] = b < n ? counts[b] : 0;
+    others[j] = shared && b < n ? shared[b] : 0;
   }
   const int64_t taken = cursor[0], given = cursor[1];
   const int64_t window = given - taken;
@@ -124,27 +127,27 @@ __global__ void __launch_bounds__(kThreads) k_kv8_plan(const int* __restrict__ p
   for (int j = 0; j < kEach; ++j) v = __builtin_elementwise_add_sat(v, max(c[j], 0));
   if (t == 0) sh.taken = sh.given = 0;
   int row = block_sums<kThreads>(v, sh.waves[0], all_rows);
-  // what each request asks for; the row offsets decide which fit the rows
+  // What each request asks for; the row offsets decide which fit the rows. (As
+  // one expression each: carried through branches, the arrays were compiled to
+  // registers that other branches had overwritten.)
   int need[kEach], give[kEach], why[kEach], needs = 0, gifts = 0;
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
     const int b = t * kEach + j;
-    need[j] = give[j] = why[j] = 0;
-    if (b >= n) continue;
-    sh.starts[b] = row;
-    sh.past[b] = p[j];
-    row = __builtin_elementwise_add_sat(row, max(c[j], 0));
-    const int64_t held = ((int64_t)p[j] + page - 1) >> shift;
-    if (p[j] < 0 || held > width) {
-      why[j] = LFM25_KV8_LENGTH;
-    } else if (c[j] < 0) {
-      give[j] = (int)held;
-    } else {
-      const int64_t after = ((int64_t)p[j] + c[j] + page - 1) >> shift;
-      if (after > width) why[j] = LFM25_KV8_TABLE;
-      else if (c[j] > 0 && row > rows) why[j] = LFM25_KV8_ROWS;
-      else need[j] = (int)(after - held);
+    if (b < n) {
+      sh.starts[b] = row;
+      sh.past[b] = p[j];
     }
+    row = __builtin_elementwise_add_sat(row, max(c[j], 0));
+    const int64_t held = ((int64_t)p[j] + page - 1) >> shift, after = ((int64_t)p[j] + max(c[j], 0) + page - 1) >> shift;
+    const bool length = p[j] < 0 || held > width || others[j] < 0 || others[j] > width || (c[j] > 0 && p[j] >> shift < others[j]);
+    why[j] = length                       ? LFM25_KV8_LENGTH
+             : c[j] < 0                   ? 0
+             : after > width              ? LFM25_KV8_TABLE
+             : c[j] > 0 && row > rows     ? LFM25_KV8_ROWS
+                                          : 0;
+    need[j] = why[j] == 0 && c[j] > 0 ? (int)(after - held) : 0;
+    give[j] = why[j] == 0 && c[j] < 0 ? max((int)held - others[j], 0) : 0;
     needs = __builtin_elementwise_add_sat(needs, need[j]);
     gifts = __builtin_elementwise_add_sat(gifts, give[j]);
   }
@@ -160,21 +163,16 @@ __global__ void __launch_bounds__(kThreads) k_kv8_plan(const int* __restrict__ p
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
     const int b = t * kEach + j;
-    if (b >= n) continue;
-    sh.takes[b] = take;
-    sh.gives[b] = back;
+    if (b < n) sh.takes[b] = take, sh.gives[b] = back;
     take = __builtin_elementwise_add_sat(take, need[j]);
     back = __builtin_elementwise_add_sat(back, give[j]);
-    if (need[j] > 0) {
-      if (take > free) why[j] = LFM25_KV8_POOL;
-      else last_take = take;
-    }
-    if (give[j] > 0) {
-      if (!sound_ring || (int64_t)free + back > ring_n) why[j] = LFM25_KV8_POOL;
-      else last_back = back;
-    }
-    sh.status[b] = (uint8_t)why[j];
-    if (first_block) status[b] = why[j], row_starts[b] = sh.starts[b];
+    const bool takes = need[j] > 0, gives = give[j] > 0;
+    const bool no = (takes && take > free) || (gives && (!sound_ring || (int64_t)free + back > ring_n));
+    last_take = takes && !no ? take : last_take;
+    last_back = gives && !no ? back : last_back;
+    const int reason = no ? LFM25_KV8_POOL : why[j];
+    if (b < n) sh.status[b] = (uint8_t)reason;
+    if (b < n && first_block) status[b] = reason, row_starts[b] = sh.starts[b];
   }
   if (last_take > 0) atomicMax(&sh.taken, last_take);
   if (last_back > 0) atomicMax(&sh.given, last_back);
@@ -195,7 +193,7 @@ __global__ void __launch_bounds__(kThreads) k_kv8_plan(const int* __restrict__ p
   }
   for (int k = me; k < returned; k += everyone) {
     const int b = last_not_above(sh.gives, n, k);
-    ring[at(tail, k)] = table[(size_t)b * width + (k - sh.gives[b])];
+    ring[at(tail, k)] = table[(size_t)b * width + (shared ? shared[b] : 0) + (k - sh.gives[b])];
   }
   if (rows <= kPlanRows || gridDim.x > 1) {
     // Four rows at a time, their page numbers asked for together. (From the
@@ -1912,10 +1910,10 @@ size_t narrow_columns(const Splits& s, int64_t kv) { return s.share > 0 ? (size_
 size_t wide_columns(const Splits& s) { return s.has_wide && s.wide > 1 ? (size_t)kWideParts * kWideColumns : 0; }
 
 template <int kThreads, int kEach>
-void plan(const lfm25_kv8_plan_call& c, int blocks, int shift, hipStream_t stream) {
+void plan(const lfm25_kv8_plan_call& c, const lfm25_kv8_plan_pages& pages, int blocks, int shift, hipStream_t stream) {
   hipLaunchKernelGGL((k_kv8_plan<kThreads, kEach>), dim3((unsigned)blocks), dim3(kThreads), sizeof(PlanShared<kThreads * kEach>), stream, c.past,
                      c.counts, c.requests, c.block_table, c.width, c.free_pages, c.ring, c.cursor, c.row_starts, c.slots, c.rows,
-                     c.next_cursor, c.status, shift);
+                     c.next_cursor, c.status, shift, pages.shared);
 }
 
 template <int D, bool kFp8, int kWaves>
@@ -1969,7 +1967,12 @@ int attend(const Attend& a, const Splits& s, hipStream_t stream) {
 using namespace lfm25;
 
 extern "C" int lfm25_kv8_plan(const lfm25_kv8_plan_call* call, lfm25_stream_t stream) {
-  LFM25_REQUIRE(call, "lfm25_kv8_plan: null pointer");
+  const lfm25_kv8_plan_pages none{};
+  return lfm25_kv8_plan_with(call, &none, stream);
+}
+
+extern "C" int lfm25_kv8_plan_with(const lfm25_kv8_plan_call* call, const lfm25_kv8_plan_pages* pages, lfm25_stream_t stream) {
+  LFM25_REQUIRE(call && pages, "lfm25_kv8_plan: null pointer");
   const lfm25_kv8_plan_call& c = *call;
   LFM25_REQUIRE(c.past && c.counts && c.block_table && c.free_pages && c.cursor && c.row_starts && c.slots && c.next_cursor && c.status,
                 "lfm25_kv8_plan: null pointer");
@@ -1978,7 +1981,7 @@ extern "C" int lfm25_kv8_plan(const lfm25_kv8_plan_call* call, lfm25_stream_t st
   LFM25_REQUIRE(c.width >= 1 && (int64_t)c.width * c.page <= INT32_MAX, "lfm25_kv8_plan: width * page must be in [1, 2^31)");
   LFM25_REQUIRE(c.ring >= 1 && c.rows >= 1, "lfm25_kv8_plan: an empty ring or no rows");
   LFM25_REQUIRE(aligned4(c.past) && aligned4(c.counts) && aligned4(c.block_table) && aligned4(c.free_pages) && aligned4(c.row_starts) &&
-                    aligned4(c.slots) && aligned4(c.status) && aligned8(c.cursor) && aligned8(c.next_cursor),
+                    aligned4(c.slots) && aligned4(c.status) && aligned8(c.cursor) && aligned8(c.next_cursor) && aligned4(pages->shared),
                 "lfm25_kv8_plan: misaligned pointer");
   const int shift = page_shift(c.page);
   // small passes with few waves to wait for one another, large ones with as
@@ -1989,11 +1992,11 @@ extern "C" int lfm25_kv8_plan(const lfm25_kv8_plan_call* call, lfm25_stream_t st
   const auto blocks = [&](int threads) {
     return in_place ? 1 : (int)std::min<int64_t>(kPlanBlocks, (c.rows + (int64_t)threads - 1) / threads);
   };
-  if (c.requests <= 64 && c.rows <= 256) plan<64, 1>(c, 1, shift, stream);
-  else if (c.requests <= 256 && (c.rows <= 1024 || !in_place)) plan<256, 1>(c, blocks(256), shift, stream);
-  else if (c.requests <= 1024 && !in_place) plan<512, 2>(c, blocks(512), shift, stream);
-  else if (c.requests <= 1024) plan<1024, 1>(c, 1, shift, stream);
-  else plan<1024, 4>(c, blocks(1024), shift, stream);
+  if (c.requests <= 64 && c.rows <= 256) plan<64, 1>(c, *pages, 1, shift, stream);
+  else if (c.requests <= 256 && (c.rows <= 1024 || !in_place)) plan<256, 1>(c, *pages, blocks(256), shift, stream);
+  else if (c.requests <= 1024 && !in_place) plan<512, 2>(c, *pages, blocks(512), shift, stream);
+  else if (c.requests <= 1024) plan<1024, 1>(c, *pages, 1, shift, stream);
+  else plan<1024, 4>(c, *pages, blocks(1024), shift, stream);
   if (c.rows > kPlanRows && in_place)
     hipLaunchKernelGGL(k_kv8_slots, dim3((unsigned)((c.rows + (int64_t)kSlotThreads - 1) / kSlotThreads)), dim3(kSlotThreads), 0, stream,
                        c.past, c.requests, c.block_table, c.width, c.row_starts, c.status, c.slots, c.rows, shift);

@@ -560,6 +560,7 @@ _KV8_MAX_REQUESTS = 4096
 _BF16, _F32, _INT32, _INT64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
 
 _PLAN = struct.Struct("@9P5i")
+_PLAN_PAGES = struct.Struct("@P")
 _APPEND = struct.Struct("@7P2q6i")
 _ATTEND = struct.Struct("@11Pq11if")
 
@@ -642,7 +643,14 @@ def _kv8_plan_check(past, counts, block_table, free_pages, cursor, row_starts, s
     _here(past, counts, block_table, free_pages, cursor, row_starts, slots, next_cursor, status)
 
 
-def kv8_plan(past, counts, block_table, free_pages, cursor, row_starts, slots, next_cursor, status, *, page: int) -> None:
+def _kv8_plan_pages(requests: int, past, shared) -> bytes:
+    _i32(shared, "shared", requests)
+    _here(past, shared)
+    return _PLAN_PAGES.pack(shared.data_ptr())
+
+
+def kv8_plan(past, counts, block_table, free_pages, cursor, row_starts, slots, next_cursor, status, *, page: int,
+             shared=None) -> None:
     """Pages, row offsets and cache slots of a pass from the requests' lengths
     (lfm25_kv8_plan). past, counts: int32 [requests], positions held and new
     rows (counts[b] < 0 ends request b and gives its pages back). block_table:
@@ -651,7 +659,12 @@ def kv8_plan(past, counts, block_table, free_pages, cursor, row_starts, slots, n
     (int64, counted on without end) are free. Written: row_starts int32
     [requests + 1], slots int32 [rows] (-1: a refused request's row, or behind
     the last), next_cursor int64 [2] (may be cursor), status int32 [requests]
-    (0, or KV8_LENGTH / KV8_TABLE / KV8_POOL / KV8_ROWS)."""
+    (0, or KV8_LENGTH / KV8_TABLE / KV8_POOL / KV8_ROWS).
+
+    A page may be in several rows of the table, but is one request's own, which
+    ends after the others that have it: shared, int32 [requests], says how many
+    pages at its beginning are not a request's own. They are neither given
+    back when it ends nor written to (lfm25_kv8_plan_with)."""
     try:
         n, ring, rows, here = past.numel(), free_pages.numel(), slots.numel(), past.get_device()
         wide = block_table.shape
@@ -672,10 +685,13 @@ def kv8_plan(past, counts, block_table, free_pages, cursor, row_starts, slots, n
         fine = False
     if not fine:
         _kv8_plan_check(past, counts, block_table, free_pages, cursor, row_starts, slots, next_cursor, status, page)
-    _lib.call("lfm25_kv8_plan", _PLAN.pack(
+    call = _PLAN.pack(
         past.data_ptr(), counts.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), cursor.data_ptr(),
-        row_starts.data_ptr(), slots.data_ptr(), next_cursor.data_ptr(), status.data_ptr(), n, wide[1], ring, rows, page),
-        _stream_of(here))
+        row_starts.data_ptr(), slots.data_ptr(), next_cursor.data_ptr(), status.data_ptr(), n, wide[1], ring, rows, page)
+    if shared is None:
+        _lib.call("lfm25_kv8_plan", call, _stream_of(here))
+    else:
+        _lib.call("lfm25_kv8_plan_with", call, _kv8_plan_pages(n, past, shared), _stream_of(here))
 
 
 def _kv8_append_check(keys, values, slots, key_cache, value_cache, key_scales, value_scales) -> None:
