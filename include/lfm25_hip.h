@@ -623,15 +623,26 @@ typedef struct lfm25_kv8_plan_call {
 } lfm25_kv8_plan_call;
 int lfm25_kv8_plan(const lfm25_kv8_plan_call* c, lfm25_stream_t stream);
 
-/* lfm25_kv8_plan() for tables that share pages. shared (int32 [requests]; NULL:
+/* lfm25_kv8_plan() for tables that share pages and lengths that go back.
+ *
+ * shared (int32 [requests]; NULL:
  * as if all 0): the first shared[b] pages of request b's row are not its own.
  * Ending, it keeps them out of the ring; new rows have to begin behind them
  * (otherwise, and where shared[b] is outside [0, width]: LFM25_KV8_LENGTH).
  * Each page is then given back once, when the request ends whose own it is:
  * let that one end after the others that have the page (until then it may
- * rest, with counts[b] = 0). */
+ * rest, with counts[b] = 0).
+ *
+ * held (int32 [requests], updated in place; NULL: what past[b] takes): the
+ * pages in request b's row of the table, those behind past[b] included. A
+ * request whose length goes back (rejected drafts) keeps its pages and fills
+ * them again before it takes others; ending, it gives all of them back, and
+ * held[b] becomes 0. held[b] has to be what past[b] takes or more, and at most
+ * width (otherwise: LFM25_KV8_LENGTH); a refused request's is left. Without
+ * it, a page that a length goes back from is lost to the ring. */
 typedef struct lfm25_kv8_plan_pages {
   const int32_t* shared;
+  int32_t* held;
 } lfm25_kv8_plan_pages;
 int lfm25_kv8_plan_with(const lfm25_kv8_plan_call* c, const lfm25_kv8_plan_pages* pages, lfm25_stream_t stream);
 

@@ -32,7 +32,7 @@ constexpr int kStatusRows = 2;  // attention: row offsets outside the rows, or m
 // (a thousand lengths and a dozen lane moves; what blocks write, none reads:
 // the ring's entries before the cursor's second counter are not given again,
 // and a request's new pages are read from the ring). Not where the cursor is
-// updated in place, which some block may still have to read: then one block,
+// (or `holds`) updated in place, which some block may still have to read: then one block,
 // and a second launch for the slots of more rows than kPlanRows (14,459 rows
 // of 1,000 requests: 8.5 + 4.2 us, in blocks of 512 threads 8.1, of 1,024
 // 8.7, of 256 9.8).
@@ -71,6 +71,7 @@ struct PlanShared {
   int takes[kMost + 1];   // pages taken before each request
   int gives[kMost + 1];   // pages given back before each request
   int past[kMost];
+  int held[kMost];  // pages of its row (where they are given)
   uint8_t status[kMost];
 };
 
@@ -98,25 +99,31 @@ __device__ __forceinline__ int block_sums(int v, int* waves, int& total) {
   return __builtin_elementwise_add_sat(before, below);
 }
 
-// kThreads threads, requests up to kEach a thread. `shared`: pages at each
-// request's beginning that are not its own (null: none).
-template <int kThreads, int kEach>
+// kThreads threads, requests up to kEach a thread. kPages, the form of
+// lfm25_kv8_plan_with() (without it 1,000 requests take 8.2 us, with the tests
+// for null pointers in it 8.6): `shared`, pages at each request's beginning that
+// are not its own (null: none); `holds`, pages in each request's row (null: what
+// its length takes), updated in place, so that one block has to do it all.
+template <int kThreads, int kEach, bool kPages>
 __global__ void __launch_bounds__(kThreads) k_kv8_plan(const int* __restrict__ past, const int* __restrict__ counts, int n,
                                                        int* table, int width, int* ring, int ring_n, const int64_t* cursor,
                                                        int* __restrict__ row_starts, int* __restrict__ slots, int rows,
                                                        int64_t* next_cursor, int* __restrict__ status, int shift,
-                                                       const int* __restrict__ shared) {
+                                                       const int* __restrict__ shared_or_null, int* holds_or_null) {
+  const int* const shared = kPages ? shared_or_null : nullptr;
+  int* const holds = kPages ? holds_or_null : nullptr;
   extern __shared__ uint4 dynamic[];
   PlanShared<kThreads * kEach>& sh = *reinterpret_cast<PlanShared<kThreads * kEach>*>(dynamic);
   const int t = threadIdx.x, page = 1 << shift, everyone = (int)gridDim.x * kThreads, me = (int)blockIdx.x * kThreads + t;
   const bool first_block = blockIdx.x == 0;
-  int p[kEach], c[kEach], others[kEach];
+  int p[kEach], c[kEach], others[kEach], had[kEach];
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
     const int b = t * kEach + j;
     p[j] = b < n ? past[b] : 0;
     c[j] = b < n ? counts[b] : 0;
     others[j] = shared && b < n ? shared[b] : 0;
+    had[j] = holds && b < n ? holds[b] : 0;
   }
   const int64_t taken = cursor[0], given = cursor[1];
   const int64_t window = given - taken;
@@ -139,14 +146,16 @@ __global__ void __launch_bounds__(kThreads) k_kv8_plan(const int* __restrict__ p
       sh.past[b] = p[j];
     }
     row = __builtin_elementwise_add_sat(row, max(c[j], 0));
-    const int64_t held = ((int64_t)p[j] + page - 1) >> shift, after = ((int64_t)p[j] + max(c[j], 0) + page - 1) >> shift;
-    const bool length = p[j] < 0 || held > width || others[j] < 0 || others[j] > width || (c[j] > 0 && p[j] >> shift < others[j]);
+    const int64_t least = ((int64_t)p[j] + page - 1) >> shift, after = ((int64_t)p[j] + max(c[j], 0) + page - 1) >> shift;
+    const int64_t held = holds ? had[j] : least;
+    if (holds && b < n) sh.held[b] = had[j];
+    const bool length = p[j] < 0 || held < least || held > width || others[j] < 0 || others[j] > width || (c[j] > 0 && p[j] >> shift < others[j]);
     why[j] = length                       ? LFM25_KV8_LENGTH
              : c[j] < 0                   ? 0
              : after > width              ? LFM25_KV8_TABLE
              : c[j] > 0 && row > rows     ? LFM25_KV8_ROWS
                                           : 0;
-    need[j] = why[j] == 0 && c[j] > 0 ? (int)(after - held) : 0;
+    need[j] = why[j] == 0 && c[j] > 0 ? max((int)(after - held), 0) : 0;
     give[j] = why[j] == 0 && c[j] < 0 ? max((int)held - others[j], 0) : 0;
     needs = __builtin_elementwise_add_sat(needs, need[j]);
     gifts = __builtin_elementwise_add_sat(gifts, give[j]);
@@ -173,6 +182,7 @@ __global__ void __launch_bounds__(kThreads) k_kv8_plan(const int* __restrict__ p
     const int reason = no ? LFM25_KV8_POOL : why[j];
     if (b < n) sh.status[b] = (uint8_t)reason;
     if (b < n && first_block) status[b] = reason, row_starts[b] = sh.starts[b];
+    if (holds && b < n && reason == 0) holds[b] = c[j] < 0 ? 0 : had[j] + need[j];
   }
   if (last_take > 0) atomicMax(&sh.taken, last_take);
   if (last_back > 0) atomicMax(&sh.given, last_back);
@@ -186,7 +196,7 @@ __global__ void __launch_bounds__(kThreads) k_kv8_plan(const int* __restrict__ p
     const int64_t i = (int64_t)from + k;
     return (int)(i >= ring_n ? i - ring_n : i);
   };
-  const auto held_by = [&](int b) { return (int)(((int64_t)sh.past[b] + page - 1) >> shift); };
+  const auto held_by = [&](int b) { return holds ? sh.held[b] : (int)(((int64_t)sh.past[b] + page - 1) >> shift); };
   for (int k = me; k < mine; k += everyone) {
     const int b = last_not_above(sh.takes, n, k);
     table[(size_t)b * width + held_by(b) + (k - sh.takes[b])] = ring[at(head, k)];
@@ -1911,9 +1921,10 @@ size_t wide_columns(const Splits& s) { return s.has_wide && s.wide > 1 ? (size_t
 
 template <int kThreads, int kEach>
 void plan(const lfm25_kv8_plan_call& c, const lfm25_kv8_plan_pages& pages, int blocks, int shift, hipStream_t stream) {
-  hipLaunchKernelGGL((k_kv8_plan<kThreads, kEach>), dim3((unsigned)blocks), dim3(kThreads), sizeof(PlanShared<kThreads * kEach>), stream, c.past,
+  const auto kernel = pages.shared || pages.held ? k_kv8_plan<kThreads, kEach, true> : k_kv8_plan<kThreads, kEach, false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), sizeof(PlanShared<kThreads * kEach>), stream, c.past,
                      c.counts, c.requests, c.block_table, c.width, c.free_pages, c.ring, c.cursor, c.row_starts, c.slots, c.rows,
-                     c.next_cursor, c.status, shift, pages.shared);
+                     c.next_cursor, c.status, shift, pages.shared, pages.held);
 }
 
 template <int D, bool kFp8, int kWaves>
@@ -1981,14 +1992,15 @@ extern "C" int lfm25_kv8_plan_with(const lfm25_kv8_plan_call* call, const lfm25_
   LFM25_REQUIRE(c.width >= 1 && (int64_t)c.width * c.page <= INT32_MAX, "lfm25_kv8_plan: width * page must be in [1, 2^31)");
   LFM25_REQUIRE(c.ring >= 1 && c.rows >= 1, "lfm25_kv8_plan: an empty ring or no rows");
   LFM25_REQUIRE(aligned4(c.past) && aligned4(c.counts) && aligned4(c.block_table) && aligned4(c.free_pages) && aligned4(c.row_starts) &&
-                    aligned4(c.slots) && aligned4(c.status) && aligned8(c.cursor) && aligned8(c.next_cursor) && aligned4(pages->shared),
+                    aligned4(c.slots) && aligned4(c.status) && aligned8(c.cursor) && aligned8(c.next_cursor) && aligned4(pages->shared) &&
+                    aligned4(pages->held),
                 "lfm25_kv8_plan: misaligned pointer");
   const int shift = page_shift(c.page);
   // small passes with few waves to wait for one another, large ones with as
   // many threads as a block has
   const uint64_t apart = c.cursor < c.next_cursor ? (uintptr_t)c.next_cursor - (uintptr_t)c.cursor
                                                   : (uintptr_t)c.cursor - (uintptr_t)c.next_cursor;
-  const bool in_place = apart < 2 * sizeof(int64_t);
+  const bool in_place = apart < 2 * sizeof(int64_t) || pages->held;
   const auto blocks = [&](int threads) {
     return in_place ? 1 : (int)std::min<int64_t>(kPlanBlocks, (c.rows + (int64_t)threads - 1) / threads);
   };

@@ -560,7 +560,7 @@ _KV8_MAX_REQUESTS = 4096
 _BF16, _F32, _INT32, _INT64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
 
 _PLAN = struct.Struct("@9P5i")
-_PLAN_PAGES = struct.Struct("@P")
+_PLAN_PAGES = struct.Struct("@2P")
 _APPEND = struct.Struct("@7P2q6i")
 _ATTEND = struct.Struct("@11Pq11if")
 
@@ -643,14 +643,16 @@ def _kv8_plan_check(past, counts, block_table, free_pages, cursor, row_starts, s
     _here(past, counts, block_table, free_pages, cursor, row_starts, slots, next_cursor, status)
 
 
-def _kv8_plan_pages(requests: int, past, shared) -> bytes:
-    _i32(shared, "shared", requests)
-    _here(past, shared)
-    return _PLAN_PAGES.pack(shared.data_ptr())
+def _kv8_plan_pages(requests: int, **pages) -> bytes:
+    for name, t in pages.items():
+        if t is not None:
+            _i32(t, name, requests)
+            _here(t)
+    return _PLAN_PAGES.pack(*(0 if t is None else t.data_ptr() for t in pages.values()))
 
 
 def kv8_plan(past, counts, block_table, free_pages, cursor, row_starts, slots, next_cursor, status, *, page: int,
-             shared=None) -> None:
+             shared=None, held=None) -> None:
     """Pages, row offsets and cache slots of a pass from the requests' lengths
     (lfm25_kv8_plan). past, counts: int32 [requests], positions held and new
     rows (counts[b] < 0 ends request b and gives its pages back). block_table:
@@ -664,7 +666,10 @@ def kv8_plan(past, counts, block_table, free_pages, cursor, row_starts, slots, n
     A page may be in several rows of the table, but is one request's own, which
     ends after the others that have it: shared, int32 [requests], says how many
     pages at its beginning are not a request's own. They are neither given
-    back when it ends nor written to (lfm25_kv8_plan_with)."""
+    back when it ends nor written to. Where lengths may go back (rejected
+    drafts), held, int32 [requests], 0 at first and updated in place, keeps the
+    pages in each row of the table; otherwise those behind a length that went
+    back are lost (lfm25_kv8_plan_with)."""
     try:
         n, ring, rows, here = past.numel(), free_pages.numel(), slots.numel(), past.get_device()
         wide = block_table.shape
@@ -688,10 +693,10 @@ def kv8_plan(past, counts, block_table, free_pages, cursor, row_starts, slots, n
     call = _PLAN.pack(
         past.data_ptr(), counts.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), cursor.data_ptr(),
         row_starts.data_ptr(), slots.data_ptr(), next_cursor.data_ptr(), status.data_ptr(), n, wide[1], ring, rows, page)
-    if shared is None:
+    if shared is None and held is None:
         _lib.call("lfm25_kv8_plan", call, _stream_of(here))
     else:
-        _lib.call("lfm25_kv8_plan_with", call, _kv8_plan_pages(n, past, shared), _stream_of(here))
+        _lib.call("lfm25_kv8_plan_with", call, _kv8_plan_pages(n, shared=shared, held=held), _stream_of(here))
 
 
 def _kv8_append_check(keys, values, slots, key_cache, value_cache, key_scales, value_scales) -> None:
