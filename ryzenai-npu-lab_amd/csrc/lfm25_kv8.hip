@@ -1,6 +1,7 @@
-// The paged 8-bit KV cache on gfx950: pages and slots for a pass (k_kv8_plan),
-// the quantizing append (k_kv8_append) and causal attention over the pages
-// (k_kv8_attend_narrow, k_kv8_attend_wide, k_kv8_combine).
+// The paged 8-bit KV cache on gfx950: pages and slots for a pass (k_kv8_plan,
+// k_kv8_slots), the quantizing append (k_kv8_append) and causal attention over
+// the pages (k_kv8_attend_narrow for few columns, k_kv8_attend_both for prompt
+// chunks and few columns beside them, k_kv8_combine).
 //
 // Layout: a pool of pages of `page` positions. Keys [pages][kv][page][dim],
 // values [pages][kv][dim][page] (a value row of one dimension is contiguous
@@ -676,15 +677,6 @@ __device__ __forceinline__ bool request_at(const Attend& a, int b, Request& r) {
   return true;
 }
 
-// The page of a request's segment that begins at position `at`, and whether
-// it may be read: a segment past the last position is not (its page number
-// may be anything), one whose number is outside the pool is not and `bad`.
-__device__ __forceinline__ int page_at(const Attend& a, const int* row, int at, int len, bool& bad) {
-  const int id = at < len ? row[at >> a.shift] : 0;
-  bad = (uint32_t)id >= (uint32_t)a.pages;
-  return bad ? 0 : id;
-}
-
 __device__ __forceinline__ float across_max16(float v) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
   const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   v = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
@@ -748,11 +740,6 @@ struct Scales {
   float ks;  // key scale * log2(e) * softmax scale
   float lv;  // log2 of the value scale; kNoValue: the values count as 0
 };
-__device__ __forceinline__ Scales scales_of(const Attend& a, size_t head, bool bad) {
-  Scales s{a.ks[head] * a.scale, scale_log2(a.vs[head])};
-  if (bad || s.lv != s.lv) s = Scales{nan_of(), kNoValue};
-  return s;
-}
 
 // The sum of two BF16 numbers and an FP32 one.
 __device__ __forceinline__ float add2(uint32_t p, float sum) {
