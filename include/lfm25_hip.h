@@ -684,7 +684,8 @@ int lfm25_kv8_append(const lfm25_kv8_append_call* c, lfm25_stream_t stream);
  * max_rows: no request brings more rows. A row that sees no position (past[b]
  * + i < 0) is zero; rows behind row_starts[requests] are left as they were. status (int32,
  * may be NULL), set and never cleared here: bit 0, a page number outside the
- * pool or a position past the table: rows that attend to it are NaN; bit 1,
+ * pool or a position past the table (or past 2^31 - 65,537): rows that attend
+ * to it are NaN; bit 1,
  * a request with row offsets outside the rows or out of order, or with more
  * than max_rows rows: its rows are left as they were. workspace:
  * lfm25_kv8_attention_workspace_bytes() of the same arguments, 16-byte

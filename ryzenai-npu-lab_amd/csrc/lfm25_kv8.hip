@@ -653,10 +653,18 @@ __device__ __forceinline__ void raise(int* status, int bit) {
 // A request as the attention takes it.
 struct Request {
   int row0, count, past;
-  int cap;  // positions that the table can hold
+  int cap;  // positions that may be attended to
   int len;  // positions that its last row sees, at most cap
   bool narrow;
 };
+
+// Positions that are attended to, of those that a table's row can stand for:
+// what the kernels look ahead of a position (a few rounds of units) is an int
+// too, and must not come out negative.
+constexpr int kMostPositions = INT32_MAX - 65535;
+__device__ __forceinline__ int positions_of(const Attend& a) {
+  return (int)min((int64_t)a.width << a.shift, (int64_t)kMostPositions);
+}
 
 __device__ __forceinline__ bool request_at(const Attend& a, int b, Request& r) {
   const int s0 = a.starts[b], s1 = a.starts[b + 1];
@@ -668,7 +676,7 @@ __device__ __forceinline__ bool request_at(const Attend& a, int b, Request& r) {
   }
   r.row0 = s0;
   r.count = s1 - s0;
-  r.cap = clamp_int((int64_t)a.width << a.shift);
+  r.cap = positions_of(a);
   const int64_t len = (int64_t)r.past + r.count;
   r.past = min(r.past, INT32_MAX - r.count);  // (past any table either way; positions stay ints)
   r.len = len < 0 ? 0 : len > r.cap ? r.cap : (int)len;
@@ -902,7 +910,7 @@ __device__ __forceinline__ bool narrow_find(const Attend& a, int at, NarrowPart&
     x.parts = uniform_of((int)mine, x.b);
     x.sp = kPart ? at - x.first : 0;
     rq.row0 = uniform_of(my.row0, x.b), rq.count = uniform_of(my.count, x.b), rq.past = uniform_of(my.past, x.b);
-    rq.len = uniform_of(my.len, x.b), rq.cap = clamp_int((int64_t)a.width << a.shift);
+    rq.len = uniform_of(my.len, x.b), rq.cap = positions_of(a);
     return x.parts > 0;
   }
   const int each = (a.requests + kWave - 1) / kWave, b0 = l * each;
@@ -1446,7 +1454,7 @@ __device__ __forceinline__ WideItem wide_find(const Attend& a, int index, bool w
     const int lane = max(x.b, 0);
     x.tile = uniform_of(upto, lane) - 1 - rank;
     rq.row0 = uniform_of(my.row0, lane), rq.count = uniform_of(my.count, lane), rq.past = uniform_of(my.past, lane);
-    rq.len = uniform_of(my.len, lane), rq.cap = clamp_int((int64_t)a.width << a.shift);
+    rq.len = uniform_of(my.len, lane), rq.cap = positions_of(a);
     return x;
   }
   const int each = (a.requests + kThreads - 1) / kThreads, b0 = threadIdx.x * each;
