@@ -690,7 +690,9 @@ int lfm25_kv8_append(const lfm25_kv8_append_call* c, lfm25_stream_t stream);
  * than max_rows rows: its rows are left as they were. workspace:
  * lfm25_kv8_attention_workspace_bytes() of the same arguments, 16-byte
  * aligned, contents ignored (NULL if that is 0); calls sharing one must not
- * overlap. output must not overlap the inputs. */
+ * overlap. (Single tokens' contexts are divided among blocks in calls of up to
+ * 256 requests; in larger ones a context is read by one block, 100,000
+ * positions in about 0.5 ms, beside a prompt in 1.3.) output must not overlap the inputs. */
 size_t lfm25_kv8_attention_workspace_bytes(int32_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim,
                                            int32_t requests, int32_t max_rows, int32_t width, int32_t page);
 typedef struct lfm25_kv8_attention_call {

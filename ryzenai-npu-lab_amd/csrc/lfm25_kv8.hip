@@ -858,7 +858,7 @@ struct NarrowShared {
 // since lengths in a batch differ as they like (a request of 100,000
 // positions beside one of 2,000: 44 us with the same number of parts for
 // each, 35 with parts of the same length).
-constexpr int kDivided = 256;  // requests, at most four a lane
+constexpr int kDivided = 256;  // requests, at most four a lane; more are not divided (see splits_for)
 struct NarrowPart {
   int b, sp;    // request and which of its parts
   int first;    // its first part among all
@@ -1155,12 +1155,12 @@ __global__ void __launch_bounds__(kWaves* kWave, D == 64 ? 4 : 2) k_kv8_attend_n
 // its own and every third (dim 64) or second (128) unit.
 //
 // What bounds it is the vector work around the products (about 280
-// instructions a unit and wave: 74,000 of a SIMD's 150,000 cycles at 3,900
+// instructions a unit and wave: 73,000 of a SIMD's 156,000 cycles at 3,900
 // rows x 16 heads of 64, the matrix cores busy for 32,000) and, in what is
 // left, the latency of one wave's chain, 2.3 us a round, and 7 us a block for
 // its beginning and its end: one tile's longest chain of units decides how
 // long a chip that holds about two tiles a CU takes. Hence the groups (one
-// group: 77 us, two: 67, three: 67 when that was measured; 61 now), the
+// group: 77 us, two: 67, three: 67 when that was measured; 60 now), the
 // halves of a round (below), and per-segment work moved out of the unit:
 // pages and scales of 64 rounds looked up at once, a lane for each (107 -> 84
 // us together with 32-bit offsets), nothing per score but the multiply-add,
@@ -1895,10 +1895,21 @@ Splits splits_for(int32_t rows, int32_t requests, int32_t kv, int32_t group, int
     s.items = requests == 1 ? 0 : s.few_tiles && requests * kv <= 128 ? 1 : (dim == 64 ? Wide<64>::kWaves : Wide<128>::kWaves) / 4;
   }
   // Single tokens: a unit takes one block 0.2 us (dim 64), and the chip's
-  // memory 0.0016 for each block; parts and their combination 4 (8 requests
-  // of 8 heads: 16.1 us whole and 15.4 in parts over 2,560 positions, 22.1 and
-  // 16.7 over 4,096; 24 requests 24.6 and 29.2). Where the memory bounds it,
-  // still in parts over long contexts, since a batch's lengths may differ.
+  // memory 0.0016 for each block; parts and their combination 4. Whole and in
+  // parts, dim 64, lengths alike (us):
+  //   blocks     1,536   2,048   2,560   3,072   4,096   5,760 positions
+  //        8  10.8 10.7  13.0 10.7  15.0 10.7  17.2 10.8  21.3 10.7  28.1 10.8
+  //       32  11.0 10.8  13.1 10.8  15.1 10.9  17.9 11.7  22.2 12.9  29.1 15.5
+  //       64  11.6 11.6  14.2 12.7  16.2 15.1  18.3 15.6  22.4 16.6  29.1 19.0
+  //       96  12.3 14.9  14.4 15.5  16.5 16.0  18.6 18.1  22.6 19.5  29.3 22.5
+  //      112  12.4 15.2  14.6 15.9  16.7 18.1  18.7 18.7  22.7 21.5  29.3 24.2
+  // and 24 requests of 8 heads, 4,096 positions, 24.6 and 29.2. The border
+  // that is taken, units * (120 - blocks) = 2,400 and none from 120 blocks on,
+  // is on the side of no parts (and of no workspace): 0 to 1.5 us at 64
+  // blocks, up to 7 at 96. Where the memory bounds it, still in parts over
+  // long contexts, since a batch's lengths may differ. More than kDivided
+  // requests are not divided at all: 256 of 1,000 positions beside one of
+  // 100,000 take 120 us, one more 559 (300 and 1,290 beside a prompt of 40).
   const int64_t target = s.has_wide ? kWideParts : full / s.waves;
   const bool many = blocks > target / 2;
   s.least = s.has_wide ? 32 : many ? 128 : s.waves;
