@@ -1897,12 +1897,12 @@ Splits splits_for(int32_t rows, int32_t requests, int32_t kv, int32_t group, int
   // Single tokens: a unit takes one block 0.2 us (dim 64), and the chip's
   // memory 0.0016 for each block; parts and their combination 4. Whole and in
   // parts, dim 64, lengths alike (us):
-  //   blocks     1,536   2,048   2,560   3,072   4,096   5,760 positions
-  //        8  10.8 10.7  13.0 10.7  15.0 10.7  17.2 10.8  21.3 10.7  28.1 10.8
-  //       32  11.0 10.8  13.1 10.8  15.1 10.9  17.9 11.7  22.2 12.9  29.1 15.5
-  //       64  11.6 11.6  14.2 12.7  16.2 15.1  18.3 15.6  22.4 16.6  29.1 19.0
-  //       96  12.3 14.9  14.4 15.5  16.5 16.0  18.6 18.1  22.6 19.5  29.3 22.5
-  //      112  12.4 15.2  14.6 15.9  16.7 18.1  18.7 18.7  22.7 21.5  29.3 24.2
+  //   blocks     1,536      2,048      2,560      4,096      5,760 positions
+  //        8  10.8 10.7  13.0 10.7  15.0 10.7  21.3 10.7  28.1 10.8
+  //       32  11.0 10.8  13.1 10.8  15.1 10.9  22.2 12.9  29.1 15.5
+  //       64  11.6 11.6  14.2 12.7  16.2 15.1  22.4 16.6  29.1 19.0
+  //       96  12.3 14.9  14.4 15.5  16.5 16.0  22.6 19.5  29.3 22.5
+  //      112  12.4 15.2  14.6 15.9  16.7 18.1  22.7 21.5  29.3 24.2
   // and 24 requests of 8 heads, 4,096 positions, 24.6 and 29.2. The border
   // that is taken, units * (120 - blocks) = 2,400 and none from 120 blocks on,
   // is on the side of no parts (and of no workspace): 0 to 1.5 us at 64
